@@ -46,7 +46,11 @@ typedef enum thrust_cdna4_dtype {
   THRUST_CDNA4_I64 = 6,
   THRUST_CDNA4_U64 = 7,
   THRUST_CDNA4_F32 = 8,
-  THRUST_CDNA4_F64 = 9
+  THRUST_CDNA4_F64 = 9,
+  /* 16-bit floating point (IEEE half, bfloat16): taken by the linear recurrence only; every other
+   * entry point refuses them. */
+  THRUST_CDNA4_F16 = 10,
+  THRUST_CDNA4_BF16 = 11
 } thrust_cdna4_dtype;
 
 /* Binary operators of thrust/functional.h that the kernels are specialised on. */
@@ -178,6 +182,145 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
                                 int num_bins, double lower, double upper, void* stream);
 
 /*
+ * Gated linear recurrence: for every channel, h[t] = a[t] * h[t-1] + x[t] along the rows of a
+ * sequence, out[t] = h[t].  It is the scan of the reference's algorithms under the composition of
+ * affine maps (a user operator over pairs there, thrust/scan.h), with 16-bit types and channels as
+ * columns.  a[t] is gate[t], or exp(gate[t]) when `log_gate` is not 0.
+ *
+ * Shapes: `batch` sequences of `rows` rows of `channels` elements; element (b, t, c) of an array is
+ * at b * batch_stride + t * row_stride + c (strides in elements, not negative).  Or packed:
+ * `offset_bytes` 4 or 8, `offsets` a DEVICE array of sequences + 1 ascending signed integers of that
+ * size, batch 1; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none.  Rows
+ * in front of the first sequence and behind the last one are part of none: their outputs are left as
+ * they were, or zero if `clear_outside` is not 0.  Offsets that do not ascend or that leave the rows
+ * give unspecified values, but no access outside the arrays.
+ *
+ * Types: x and out are F32, F16 or BF16; the gates are of the same type or F32.  Arithmetic and
+ * states are in 32 bits; out is rounded once.  `init` (NULL: zero) and `final_state` (NULL: not
+ * wanted) are F32 [sequences or batch][channels], contiguous, and must not overlap; a sequence without
+ * rows passes its state on.  `states` (NULL: not wanted) is F32
+ * [batch][ceil(rows / THRUST_CDNA4_LINEAR_SCAN_CHUNK)][channels]: the state that enters each chunk of
+ * rows, which the gradient needs.  out may be x or gate itself (same address, strides and type); any
+ * other overlap of an output with an input is an error that is not detected.
+ *
+ * Infinities and NaNs stay in their channel and sequence.  Products of factors over up to 512 rows are
+ * formed on their own: where one underflows, an infinite state turns into NaN; where one overflows
+ * 32 bits, a state of zero does.  Results are the same from run to run: what
+ * is combined with what depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan.
+ */
+#define THRUST_CDNA4_LINEAR_SCAN_CHUNK 64
+typedef struct thrust_cdna4_linear_scan_args {
+  int gate_dtype, x_dtype, log_gate, offset_bytes, clear_outside;
+  int64_t batch, rows, channels, sequences;
+  const void* gate;
+  int64_t gate_batch_stride, gate_row_stride;
+  const void* x;
+  int64_t x_batch_stride, x_row_stride;
+  void* out;
+  int64_t out_batch_stride, out_row_stride;
+  const void* offsets;
+  const void* init;
+  void* final_state;
+  void* states;
+} thrust_cdna4_linear_scan_args;
+int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const thrust_cdna4_linear_scan_args* args, void* stream);
+
+/*
+ * Its gradient.  From grad_out (the type of x) and `grad_final` (F32, NULL: zero) computes grad_x (the
+ * type of x), grad_gate (the type of gate; for log_gate the gradient of the logarithm) and `grad_init`
+ * (F32 [sequences or batch][channels], NULL: not wanted; must not overlap init or grad_final), with the
+ * recurrence's inputs and the `states` it left.
+ */
+typedef struct thrust_cdna4_linear_scan_backward_args {
+  int gate_dtype, x_dtype, log_gate, offset_bytes, clear_outside;
+  int64_t batch, rows, channels, sequences;
+  const void* gate;
+  int64_t gate_batch_stride, gate_row_stride;
+  const void* x;
+  int64_t x_batch_stride, x_row_stride;
+  const void* grad_out;
+  int64_t grad_out_batch_stride, grad_out_row_stride;
+  void* grad_gate;
+  int64_t grad_gate_batch_stride, grad_gate_row_stride;
+  void* grad_x;
+  int64_t grad_x_batch_stride, grad_x_row_stride;
+  const void* offsets;
+  const void* init;
+  const void* states;
+  const void* grad_final;
+  void* grad_init;
+} thrust_cdna4_linear_scan_backward_args;
+int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes, const thrust_cdna4_linear_scan_backward_args* args, void* stream);
+
+/*
+ * One row for each of `batch` sequences, against states kept between calls: for row i with
+ * s = slots[i] (NULL: s = i), state[s] = a[i] * state[s] + x[i] and out[i] = state[s].  `state` is F32
+ * [num_slots][channels], contiguous, updated in place; `slots` a DEVICE array.  A row whose slot is
+ * negative or not below num_slots is padding: its out is zero and no state changes.  Rows of one slot
+ * are successive tokens of one sequence and taken in their order.  Needs no temporary storage.  The
+ * arrays must not overlap, except that out may be x or gate itself.
+ */
+int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, const void* gate, int64_t gate_row_stride,
+                                  const void* x, int64_t x_row_stride, void* out, int64_t out_row_stride, void* state,
+                                  int64_t num_slots, const int32_t* slots, int64_t batch, int64_t channels, void* stream);
+
+/*
+ * Pages of a cache.  A cache is `num_pools` arrays of `num_pages` pages of `page_bytes` bytes (a layer's
+ * keys, its values, its recurrent states ...), of which page q of every pool belongs together; tables,
+ * which say for each of `num_sequences` sequences the pages that hold its tokens, `page_size` tokens a
+ * page; and refs, which count how many tables name a page.  A page of count 0 is free; there is no
+ * list of free pages.  Everything is in device memory, nothing is read back, and a call's effect
+ * depends on the contents of these arrays alone, so calls can be captured and replayed.
+ *
+ * `pools` is a DEVICE array of the pools' device addresses (any alignment).  tables is
+ * [num_sequences][max_pages], -1 behind a sequence's pages.  A length is a number of tokens; a sequence
+ * of length n holds the first ceil(n / page_size) entries of its row.
+ *
+ * Requests of a call are served as if in their order: each in turn takes the lowest free pages.  One
+ * that cannot be served leaves everything of its sequence as it was and has done[i] = 0, and so has
+ * one with an id out of range or a sequence that an earlier request of the call names already.  One
+ * that needs pages is refused when the pages wanted by it and by all requests before it (refused ones
+ * among them) are more than there were free.  Entries of a table that name no page are passed over.
+ */
+typedef struct thrust_cdna4_page_cache {
+  const uint64_t* pools;
+  int64_t page_bytes;
+  int32_t num_pools, num_pages, page_size, num_sequences, max_pages;
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* refs;
+} thrust_cdna4_page_cache;
+
+/*
+ * Sequence children[i], which must be empty and must not be a parent in the call, becomes a copy of
+ * parents[i].  share != 0: it names the parent's full pages too (their counts rise) and gets a copy of
+ * the partly filled last one, if there is one.  share == 0: it gets copies of all.
+ */
+int thrust_cdna4_pages_fork(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, const int32_t* parents,
+                            const int32_t* children, int64_t n, int share, uint8_t* done, void* stream);
+
+/*
+ * sequences[i] gets the length lengths[i].  Pages that shrinking
+ * sequences give up are there for the growing ones of the same call.  A growing sequence whose last
+ * page is partly filled and named by others too gets a copy of that page, so that what is appended is
+ * its own.  A length that is negative or over max_pages * page_size is refused.
+ */
+int thrust_cdna4_pages_resize(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, const int32_t* sequences,
+                              const int32_t* lengths, int64_t n, uint8_t* done, void* stream);
+
+/* The sequences give back all their pages: resize to length 0, without temporary storage.  `done` may be NULL. */
+int thrust_cdna4_pages_free(const thrust_cdna4_page_cache* cache, const int32_t* sequences, int64_t n, uint8_t* done, void* stream);
+
+/*
+ * Moves pages until those in use are the lowest: the highest page in use moves to the lowest free one,
+ * and so on.  Writes the renumbered tables and refs to tables_out and refs_out, which may be those
+ * of the cache, and the number of pages in use to live_out (DEVICE, int32).  The pages moved from keep
+ * their contents: work in flight with the old tables may end.
+ */
+int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, int32_t* tables_out,
+                               int32_t* refs_out, int32_t* live_out, void* stream);
+
+/*
  * Temporary-storage allocator.  Replaces cuda_cub::malloc / cuda_cub::free
  * (thrust/system/cuda/detail/malloc_and_free.h:53-116), which call cudaMalloc / cudaFree on
  * every algorithm invocation.  Blocks are cached per device in size classes (powers of two up
@@ -303,7 +446,7 @@ int thrust_cdna4_profile_get(int index, const char** name, float* ms);
 int thrust_cdna4_sort_status(const void* temp, int64_t n, void* stream);
 /*
  * Diagnostics; no counterpart in the reference.  Counts the waits that did not end (see
- * thrust_cdna4_sort_status) per device: blocks until the device is idle and stores the count
+ * thrust_cdna4_sort_status; those of the linear recurrence among them) per device: blocks until the device is idle and stores the count
  * since the process started; anything but 0 means that some sort's result cannot be trusted.
  */
 int thrust_cdna4_lookback_timeouts(unsigned long long* count);

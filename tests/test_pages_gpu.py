@@ -1,0 +1,402 @@
+"""The page cache on the GPU against the same operations on lists."""
+import random
+
+import pytest
+import torch
+
+import thrust_amd
+from lm_util import get, put
+
+pytestmark = pytest.mark.gpu
+
+
+class Lists:
+    """The definitions: one request after the other, one page after the other."""
+
+    def __init__(self, pools, page_size, tables, lengths, refs):
+        self.size, self.most = page_size, tables.shape[1]
+        self.pools = [p.clone() for p in pools]
+        self.tables = tables.tolist()
+        self.lengths, self.refs = lengths.tolist(), refs.tolist()
+
+    def held(self, n):
+        return -(-n // self.size)
+
+    def copy(self, pairs):
+        for pool in self.pools:
+            old = pool.clone()
+            for a, b in pairs:
+                pool[b] = old[a]
+
+    def valid(self, s):
+        return 0 <= s < len(self.lengths)
+
+    def free(self, sequences):
+        self.resize(sequences, [0] * len(sequences), free_only=True)
+
+    def resize(self, sequences, lengths, free_only=False):
+        n = len(sequences)
+        ok = [self.valid(s) and 0 <= want <= self.most * self.size and s not in sequences[:i] for i, (s, want) in enumerate(zip(sequences, lengths))]
+        for i in range(n):
+            s = sequences[i]
+            if ok[i] and lengths[i] < self.lengths[s]:
+                for j in range(self.held(lengths[i]), self.held(self.lengths[s])):
+                    if 0 <= self.tables[s][j] < len(self.refs):
+                        self.refs[self.tables[s][j]] -= 1
+                    self.tables[s][j] = -1
+                self.lengths[s] = lengths[i]
+        if free_only:
+            return ok
+        free = [p for p, r in enumerate(self.refs) if r == 0]
+        at, copies, refs = 0, [], list(self.refs)
+        for i in range(n):
+            if not ok[i]:
+                continue
+            s, want = sequences[i], lengths[i]
+            had, have = self.held(self.lengths[s]), self.held(want)
+            if want <= self.lengths[s]:
+                continue
+            last = self.tables[s][self.lengths[s] // self.size] if self.lengths[s] % self.size else -1
+            own = 0 <= last < len(refs) and refs[last] > 1
+            need = have - had + own
+            mine = free[at:at + need]
+            at += need
+            if len(mine) < need:
+                ok[i] = False
+                continue
+            if own:
+                copies.append((last, mine[0]))
+                self.refs[last] -= 1
+                self.refs[mine[0]] = 1
+                self.tables[s][self.lengths[s] // self.size] = mine[0]
+                mine = mine[1:]
+            for j, p in enumerate(mine):
+                self.tables[s][had + j] = p
+                self.refs[p] = 1
+            self.lengths[s] = want
+        self.copy(copies)
+        return ok
+
+    def fork(self, parents, children, share):
+        free = [p for p, r in enumerate(self.refs) if r == 0]
+        at, copies, ok, before = 0, [], [], list(self.lengths)
+        for i, (p, c) in enumerate(zip(parents, children)):
+            good = self.valid(p) and self.valid(c) and before[c] == 0 and c not in children[:i] and c not in parents
+            if good:
+                n = self.lengths[p]
+                held = self.held(n)
+                need = (1 if n % self.size else 0) if share else held
+                mine = free[at:at + need]
+                at += need
+                good = len(mine) == need
+                if good:
+                    for j in range(held):
+                        q = self.tables[p][j]
+                        if j < held - need:
+                            if 0 <= q < len(self.refs):
+                                self.refs[q] += 1
+                        else:
+                            new = mine[j - held + need]
+                            if 0 <= q < len(self.refs):
+                                copies.append((q, new))
+                            q = new
+                            self.refs[q] = 1
+                        self.tables[c][j] = q
+                    self.lengths[c] = n
+            ok.append(good)
+        self.copy(copies)
+        return ok
+
+    def compact(self):
+        live = sum(r > 0 for r in self.refs)
+        holes = [p for p in range(live) if self.refs[p] == 0]
+        high = [p for p in range(len(self.refs) - 1, live - 1, -1) if self.refs[p] > 0]
+        self.copy(list(zip(high, holes)))
+        names = dict(zip(high, holes))
+        for a, b in names.items():
+            self.refs[b], self.refs[a] = self.refs[a], 0
+        self.tables = [[names.get(q, q) if 0 <= q < len(self.refs) else -1 for q in row] for row in self.tables]
+        return live
+
+
+def ints(v):
+    return put(torch.tensor(v, dtype=torch.int32))
+
+
+def make(pages, shapes, page_size, sequences, most, seed=1, unaligned=False):
+    g = torch.Generator().manual_seed(seed)
+    pools = []
+    for shape, dtype in shapes:
+        v = torch.randint(-100, 100, (pages,) + shape, generator=g).to(dtype)
+        pools.append(v)
+    on = [put(torch.cat([v.flatten()[:1], v.flatten()]))[1:].view(v.shape) if unaligned else put(v) for v in pools]
+    cache = thrust_amd.PageCache(on, page_size, sequences, most)
+    return cache, Lists(pools, page_size, get(cache.tables), get(cache.lengths), get(cache.refs))
+
+
+def same(cache, ref):
+    assert get(cache.tables).tolist() == ref.tables
+    assert get(cache.lengths).tolist() == ref.lengths
+    assert get(cache.refs).tolist() == ref.refs
+    for a, b in zip(cache.pools, ref.pools):
+        assert torch.equal(get(a), b)
+
+
+POOLS = {
+    "states": [((5,), torch.float32)] * 3,
+    "keys and values": [((4, 2, 8), torch.bfloat16)] * 4,
+    "odd bytes": [((13,), torch.int8)] * 2,
+    "one byte": [((1,), torch.uint8)],
+    "over a copy unit": [((4100, 1), torch.float32), ((2, 2050), torch.int32)],
+    "no bytes": [((0,), torch.float32)],
+}
+
+
+@pytest.mark.parametrize("pools", list(POOLS), ids=str)
+@pytest.mark.parametrize("page_size,most,unaligned", [(16, 6, False), (1, 9, True), (1 << 20, 1, False), (7, 4, True)])
+def test_life_of_a_cache(pools, page_size, most, unaligned):
+    """Random requests, valid and not, until pages have run out and come back many times."""
+    rng = random.Random(len(pools) * 100 + page_size)
+    pages, sequences = (23, 11) if pools == "over a copy unit" else (70, 25)
+    cache, ref = make(pages, POOLS[pools], page_size, sequences, most, unaligned=unaligned)
+    cap, refused, copied = page_size * most, 0, 0
+    for turn in range(8 if pools == "over a copy unit" else 30):
+        n = rng.choice([1, 2, 5, 9])
+        ids = [rng.randrange(sequences) for _ in range(n)]
+        if rng.random() < 0.5:
+            ids[0] = rng.choice([-1, sequences, 2 ** 31 - 1, -2 ** 31, ids[-1]])
+        what = rng.choice(["resize", "resize", "resize", "fork", "fork", "copy", "free", "compact"])
+        if what == "resize":
+            lengths = [rng.choice([rng.randint(0, cap), min(cap, ref.lengths[s] + 1) if 0 <= s < sequences else 3]) for s in ids]
+            if rng.random() < 0.2:
+                lengths[-1] = rng.choice([-1, cap + 1, -2 ** 31, 2 ** 31 - 1])
+            done = get(cache.resize(ints(ids), ints(lengths))).tolist()
+            assert done == ref.resize(ids, lengths)
+            refused += not all(done)
+        elif what in ("fork", "copy"):
+            empty = [s for s in range(sequences) if ref.lengths[s] == 0]
+            rng.shuffle(empty)
+            children = (empty + ids)[:n]
+            used = [s for s in range(sequences) if ref.lengths[s]] or [0]
+            parents = [rng.choice(used + [rng.randrange(-1, sequences + 1)]) for _ in range(n)]
+            done = get(cache.fork(ints(parents), ints(children), share=what == "fork")).tolist()
+            assert done == ref.fork(parents, children, what == "fork")
+            copied += any(done)
+        elif what == "free":
+            cache.free(ints(ids))
+            ref.free(ids)
+        else:
+            assert get(cache.compact()).tolist() == [ref.compact()]
+        same(cache, ref)
+    assert sum(r > 0 for r in ref.refs) == len({q for row in ref.tables for q in row if q >= 0})
+
+
+def test_fork_shares_full_pages_and_growth_copies_a_shared_one():
+    cache, ref = make(20, [((16, 2), torch.float32)], 16, 6, 4)
+    for c in (cache, ref):
+        c.resize(*((ints(v) if c is cache else v) for v in ([0], [40])))
+    assert get(cache.tables)[0].tolist() == [0, 1, 2, -1]
+    cache.fork(ints([0, 0]), ints([1, 2]))
+    ref.fork([0, 0], [1, 2], True)
+    same(cache, ref)
+    assert get(cache.refs)[:5].tolist() == [3, 3, 1, 1, 1]
+    # cut back into a shared page: it is copied when the sequences grow again, in the order of the requests
+    for ids, lengths in (([0, 1, 2], [20, 20, 20]), ([1, 0], [21, 33])):
+        assert get(cache.resize(ints(ids), ints(lengths))).tolist() == ref.resize(ids, lengths) == [True] * len(ids)
+        same(cache, ref)
+    assert get(cache.tables)[:3, :2].tolist() == [[0, 3], [0, 2], [0, 1]] and get(cache.refs)[1] == 1
+
+
+def test_requests_are_served_in_order_and_whole():
+    cache, ref = make(10, [((3,), torch.float32)], 4, 5, 8)
+    ids, lengths = [3, 1, 0, 4], [13, 30, 9, 8]  # 4, 8, 3, 2 pages: what all requests up to one want counts
+    done = get(cache.resize(ints(ids), ints(lengths))).tolist()
+    assert done == ref.resize(ids, lengths) == [True, False, False, False]
+    same(cache, ref)
+    assert get(cache.resize(ints([1, 3]), ints([24, 0]))).tolist() == [True, True]  # pages given up in the call count
+    assert get(cache.tables)[1].tolist() == [0, 1, 2, 3, 4, 5, -1, -1]
+    assert get(cache.fork(ints([1, 1]), ints([0, 1]), share=False)).tolist() == [False, False]  # 4 pages for 6; not empty
+    assert get(cache.refs).tolist() == [1] * 6 + [0] * 4
+
+
+def test_tables_that_name_no_page():
+    tables = torch.tensor([[5, 99, -7, 2], [-1, -1, -1, -1], [1, 2 ** 31 - 1, -2 ** 31, 9]], dtype=torch.int32)
+    lengths = torch.tensor([15, 0, 13], dtype=torch.int32)
+    refs = torch.tensor([0, 1, 1, 0, 0, 1, 0, 0, 0, 1, 0, 0], dtype=torch.int32)
+    for op in range(4):
+        pools = [torch.arange(36.0).view(12, 3)]
+        cache = thrust_amd.PageCache([put(pools[0])], 4, 3, 4, tables=put(tables), lengths=put(lengths), refs=put(refs))
+        ref = Lists(pools, 4, tables, lengths, refs)
+        if op < 2:
+            assert get(cache.fork(ints([0]), ints([1]), share=op == 0)).tolist() == ref.fork([0], [1], op == 0)
+        elif op == 2:
+            assert get(cache.resize(ints([2, 0]), ints([14, 2]))).tolist() == ref.resize([2, 0], [14, 2])
+        else:
+            assert get(cache.compact()).tolist() == [ref.compact()]
+        same(cache, ref)
+
+
+def test_lengths_out_of_range_are_taken_as_the_nearest():
+    pools = [torch.arange(24.0).view(8, 3)]
+    tables = torch.tensor([[0, 1], [2, -1], [-1, -1]], dtype=torch.int32)
+    refs = torch.tensor([1, 1, 1, 0, 0, 0, 0, 0], dtype=torch.int32)
+    cache = thrust_amd.PageCache([put(pools[0])], 4, 3, 2, tables=put(tables), lengths=ints([2 ** 31 - 1, -5, 0]), refs=put(refs))
+    assert get(cache.fork(ints([0, 1]), ints([2, 1]))).tolist() == [True, False]  # -5 is not empty, as a child
+    assert get(cache.tables).tolist() == [[0, 1], [2, -1], [0, 1]] and get(cache.lengths).tolist() == [2 ** 31 - 1, -5, 8]
+    cache.free(ints([0]))
+    assert get(cache.refs).tolist() == [1, 1, 1, 0, 0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("pages", [1, 2047, 2048, 2049, 10000])
+@pytest.mark.parametrize("live", [0.0, 0.3, 0.97, 1.0])
+def test_compact_many_pages(pages, live):
+    g = torch.Generator().manual_seed(pages)
+    refs = (torch.rand(pages, generator=g) < live).int() * torch.randint(1, 4, (pages,), generator=g).int()
+    used = refs.nonzero().flatten().int()
+    sequences, most = 37, 50
+    tables = torch.full((sequences, most), -1, dtype=torch.int32)
+    if len(used):
+        tables = used[torch.randint(0, len(used), (sequences, most), generator=g)]
+    lengths = torch.full((sequences,), most, dtype=torch.int32)
+    pool = torch.arange(pages * 2).view(pages, 2)
+    ref = Lists([pool], 1, tables, lengths, refs)
+    n = ref.compact()
+    apart = thrust_amd.PageCache([put(pool)], 1, sequences, most, tables=put(tables), lengths=put(lengths), refs=put(refs))
+    new_tables, new_refs = put(torch.zeros_like(tables)), put(torch.full_like(refs, 77))
+    assert get(apart.compact(tables=new_tables, refs=new_refs)).tolist() == [n]
+    assert get(new_tables).tolist() == ref.tables and get(new_refs).tolist() == ref.refs and torch.equal(get(apart.pools[0]), ref.pools[0])
+    assert torch.equal(get(apart.tables), tables) and torch.equal(get(apart.refs), refs)  # the old ones stand ...
+    old = pool[tables.long().clamp(min=0)]
+    moved = torch.isin(tables, torch.arange(n, dtype=torch.int32), invert=True)
+    assert torch.equal(get(apart.pools[0])[tables.long().clamp(min=0)][moved], old[moved])  # ... and so does what they name
+    here = thrust_amd.PageCache([put(pool)], 1, sequences, most, tables=put(tables), lengths=put(lengths), refs=put(refs))
+    assert get(here.compact()).tolist() == [n]
+    same(here, ref)
+
+
+@pytest.mark.parametrize("requests", [300, 1100])
+def test_fork_and_resize_many_requests(requests):
+    sequences = 2 * requests
+    cache, ref = make(3 * requests + 50, [((1,), torch.int32)], 4, sequences, 3)
+    rng = random.Random(requests)
+    ids = list(range(sequences))
+    rng.shuffle(ids)
+    lengths = [rng.randint(0, 12) for _ in range(requests)]
+    first, second = ids[:requests], ids[requests:]
+    for call in range(3):
+        if call == 0:
+            a, b = get(cache.resize(ints(first), ints(lengths))).tolist(), ref.resize(first, lengths)
+        elif call == 1:
+            a, b = get(cache.fork(ints(first), ints(second))).tolist(), ref.fork(first, second, True)
+        else:
+            a, b = get(cache.resize(ints(ids), ints([2] * sequences))).tolist(), ref.resize(ids, [2] * sequences)
+        assert a == b
+        same(cache, ref)
+
+
+def test_nothing_to_do():
+    cache, ref = make(0, [((3,), torch.float32)], 4, 3, 2)
+    assert get(cache.resize(ints([0, 1]), ints([0, 1]))).tolist() == [True, False]
+    assert get(cache.fork(ints([0]), ints([1]))).tolist() == [True]
+    assert get(cache.compact()).tolist() == [0]
+    cache, ref = make(5, [((3,), torch.float32)], 4, 3, 2)
+    none = put(torch.zeros(0, dtype=torch.int32))
+    assert get(cache.resize(none, none)).tolist() == [] and get(cache.fork(none, none)).tolist() == []
+    cache.free(none)
+    assert get(cache.compact()).tolist() == [0]
+    same(cache, ref)
+    cache, ref = make(5, [((3,), torch.float32)], 4, 0, 0)
+    assert get(cache.resize(ints([0]), ints([1]))).tolist() == [False]
+    assert get(cache.compact()).tolist() == [0]
+
+
+def test_states_of_a_recurrence_in_a_cache():
+    """Prompts are scanned, their last states kept in pages, sequences forked and continued token by token, closed up in between: the
+    outputs are those of one scan over each whole sequence."""
+    channels, prompts, tokens = 132, [5, 1, 70], 6
+    g = torch.Generator().manual_seed(5)
+    pool = put(torch.zeros(9, channels))
+    cache = thrust_amd.PageCache([pool], 1 << 20, 5, 1)
+
+    def rows(n):
+        return torch.rand(n, channels, generator=g).bfloat16(), torch.randn(n, channels, generator=g).bfloat16()
+    gate, x = rows(sum(prompts))
+    offsets = torch.tensor([0] + prompts).cumsum(0).int()
+    # a page that is given back leaves a hole for the compaction
+    assert get(cache.resize(ints([4, 0, 1, 2]), ints([1] + prompts))).all()
+    cache.free(ints([4]))
+    out, final = thrust_amd.linear_scan(put(gate), put(x), offsets=put(offsets))
+    pool[cache.tables[:3, 0].long()] = final
+    histories = [[gate[a:b], x[a:b]] for a, b in zip(offsets[:-1].tolist(), offsets[1:].tolist())]
+    assert get(cache.fork(ints([2, 2]), ints([3, 4]))).all()
+    histories += [[v.clone() for v in histories[2]] for _ in range(2)]
+    got = [[] for _ in range(5)]
+    for t in range(tokens):
+        if t == 3:
+            assert get(cache.compact()).tolist() == [5]
+        gate, x = rows(5)
+        slots = cache.tables[:, 0].contiguous()
+        assert t < 3 or sorted(get(slots).tolist()) == list(range(5))
+        step = get(thrust_amd.linear_scan_step(put(gate), put(x), pool, slots=slots))
+        for s in range(5):
+            histories[s] = [torch.cat([a, b[s:s + 1]]) for a, b in zip(histories[s], (gate, x))]
+            got[s].append(step[s])
+    for s in range(5):
+        want, final = thrust_amd.linear_scan(put(histories[s][0][None]), put(histories[s][1][None]))
+        tail = get(want)[0, -tokens:].float()
+        # both are within the bound of a 32-bit sum of the exact value, then rounded: at most one step apart, relative to the
+        # largest value that the sum of at most 76 terms below 5 can have met (1e-3 absolute covers 2 * 80 roundings of 2^-24 * 100)
+        assert ((torch.stack(got[s]).float() - tail).abs() <= torch.finfo(torch.bfloat16).eps * tail.abs() + 1e-3).all()
+
+
+@pytest.mark.needs_device
+def test_requests_in_a_graph():
+    cache, ref = make(400, [((64,), torch.float32)] * 2, 4, 40, 12)
+    ids, lengths = put(torch.arange(10).int()), put(torch.full((10,), 9).int())
+    parents, children = put(torch.zeros(5).int()), put(torch.arange(20, 25).int())
+
+    def one():
+        cache.free(children)
+        done = cache.resize(ids, lengths)
+        forked = cache.fork(parents, children)
+        return done, forked, cache.compact()
+    one()
+    cache.free(put(torch.arange(40).int()))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = one()
+    ref.pools = [get(p) for p in cache.pools]
+    rng = random.Random(2)
+    for r in range(5):
+        a = rng.sample(range(20), 10)
+        b = [rng.randint(0, 48) for _ in range(10)]
+        p = [rng.choice(a) for _ in range(5)]
+        ids.copy_(torch.tensor(a).int())
+        lengths.copy_(torch.tensor(b).int())
+        parents.copy_(torch.tensor(p).int())
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        ref.free(list(range(20, 25)))
+        want = ref.resize(a, b), ref.fork(p, list(range(20, 25)), True), [ref.compact()]
+        assert [get(o).tolist() for o in outs] == list(want)
+        same(cache, ref)
+
+
+@pytest.mark.needs_device
+def test_pools_past_4_gib():
+    pages, width = 70000, 20000  # 5.6 GB of float32
+    pool = torch.zeros((pages, width), device="cuda")
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    cache = thrust_amd.PageCache([pool], 1 << 20, 4, 1, refs=refs)
+    refs[: pages - 1] = 1  # of no table: only the last page is free
+    assert get(cache.resize(ints([0]), ints([3]))).all()
+    assert get(cache.tables)[0, 0] == pages - 1
+    pool[pages - 1] = torch.arange(width, device="cuda").float()
+    refs[5:pages - 1] = 0
+    assert get(cache.fork(ints([0]), ints([1]))).all() and get(cache.tables)[1, 0] == 5
+    assert get(cache.compact()).tolist() == [7]
+    assert get(cache.tables)[:2, 0].tolist() == [6, 5]
+    want = torch.arange(width).float()
+    assert torch.equal(get(pool[5]), want) and torch.equal(get(pool[6]), want)

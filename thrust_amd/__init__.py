@@ -8,3 +8,5 @@ the C ABI on torch-owned device memory; torch supplies allocations and streams o
 from . import capi  # noqa: F401
 from .api import (exclusive_scan, exclusive_scan_by_key, histogram_even,  # noqa: F401
                   inclusive_scan, inclusive_scan_by_key, reduce_by_key, sort, sort_by_key)
+from .pages import PageCache  # noqa: F401
+from .recurrence import linear_scan, linear_scan_backward, linear_scan_step  # noqa: F401

@@ -9,7 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # THRUST_CDNA4_LIB points the harness at another build of the same C ABI (tuning builds).
 LIB_PATH = os.environ.get("THRUST_CDNA4_LIB") or os.path.join(_HERE, "lib", "libthrust_cdna4.so")
 
-I8, U8, I16, U16, I32, U32, I64, U64, F32, F64 = range(10)
+I8, U8, I16, U16, I32, U32, I64, U64, F32, F64, F16, BF16 = range(12)
 PLUS, MULTIPLIES, MAXIMUM, MINIMUM = range(4)
 
 # every symbol include/thrust_cdna4.h declares
@@ -31,7 +31,37 @@ SYMBOLS = [
     "thrust_cdna4_selftest_xcd_dispatch", "thrust_cdna4_set_test_sort_plain_tickets",
     "thrust_cdna4_sort_status", "thrust_cdna4_set_test_sort_spin_limit", "thrust_cdna4_sort_tile_assignment",
     "thrust_cdna4_lookback_timeout_counter",
+    "thrust_cdna4_linear_scan", "thrust_cdna4_linear_scan_backward", "thrust_cdna4_linear_scan_step",
+    "thrust_cdna4_pages_fork", "thrust_cdna4_pages_resize", "thrust_cdna4_pages_free", "thrust_cdna4_pages_compact",
 ]
+
+LINEAR_SCAN_CHUNK = 64  # THRUST_CDNA4_LINEAR_SCAN_CHUNK
+
+
+def _strided(*names):
+    return [f for n in names for f in ((n, ctypes.c_void_p), (n + "_batch_stride", ctypes.c_int64), (n + "_row_stride", ctypes.c_int64))]
+
+
+_SHAPE = [(n, ctypes.c_int) for n in ("gate_dtype", "x_dtype", "log_gate", "offset_bytes", "clear_outside")] + \
+         [(n, ctypes.c_int64) for n in ("batch", "rows", "channels", "sequences")]
+
+
+class LinearScanArgs(ctypes.Structure):
+    """thrust_cdna4_linear_scan_args"""
+    _fields_ = _SHAPE + _strided("gate", "x", "out") + [(n, ctypes.c_void_p) for n in ("offsets", "init", "final_state", "states")]
+
+
+class LinearScanBackwardArgs(ctypes.Structure):
+    """thrust_cdna4_linear_scan_backward_args"""
+    _fields_ = _SHAPE + _strided("gate", "x", "grad_out", "grad_gate", "grad_x") + \
+        [(n, ctypes.c_void_p) for n in ("offsets", "init", "states", "grad_final", "grad_init")]
+
+
+class PageCacheArgs(ctypes.Structure):
+    """thrust_cdna4_page_cache"""
+    _fields_ = [("pools", ctypes.c_void_p), ("page_bytes", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("num_pools", "num_pages", "page_size", "num_sequences", "max_pages")] + \
+        [(n, ctypes.c_void_p) for n in ("tables", "lengths", "refs")]
 
 
 class Cdna4Error(RuntimeError):
@@ -65,6 +95,14 @@ def bind(path):
     L.thrust_cdna4_scan_by_key.argtypes = [vp, psz, i32, i32, i32, i32, vp, vp, vp, i64, vp, vp]
     L.thrust_cdna4_reduce_by_key.argtypes = [vp, psz, i32, i32, i32, vp, vp, vp, vp, vp, i64, vp]
     L.thrust_cdna4_histogram_even.argtypes = [vp, psz, i32, vp, i64, vp, i32, dbl, dbl, vp]
+    L.thrust_cdna4_linear_scan.argtypes = [vp, psz, ctypes.POINTER(LinearScanArgs), vp]
+    L.thrust_cdna4_linear_scan_backward.argtypes = [vp, psz, ctypes.POINTER(LinearScanBackwardArgs), vp]
+    L.thrust_cdna4_linear_scan_step.argtypes = [i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, i64, vp]
+    cache = ctypes.POINTER(PageCacheArgs)
+    L.thrust_cdna4_pages_fork.argtypes = [vp, psz, cache, vp, vp, i64, i32, vp, vp]
+    L.thrust_cdna4_pages_resize.argtypes = [vp, psz, cache, vp, vp, i64, vp, vp]
+    L.thrust_cdna4_pages_free.argtypes = [cache, vp, i64, vp, vp]
+    L.thrust_cdna4_pages_compact.argtypes = [vp, psz, cache, vp, vp, vp, vp]
     L.thrust_cdna4_malloc.argtypes = [ctypes.POINTER(vp), sz, vp]
     L.thrust_cdna4_free.argtypes = [vp, vp]
     L.thrust_cdna4_pool_bytes.restype = sz

@@ -1,0 +1,962 @@
+// Gated linear recurrence for gfx950: h[t] = a[t] h[t-1] + x[t] for every channel, its gradient, and
+// the step of single tokens against a cache of states.
+//
+// Mathematics.  Row t is the affine map m_t(h) = a_t h + x_t; the maps of consecutive rows compose to
+// a map of the same form, (A, H) after (A', H') = (A A', A H' + H), and composition is associative, so
+// the recurrence is a scan along the rows, independent for every channel.  The gradient is the same
+// scan from the last row to the first: with c the gradient of the state that enters row t + 1,
+//   g_t = dout_t + c,  dx_t = g_t,  da_t = g_t h_{t-1} (times a_t when the gate is a logarithm),
+//   c <- a_t g_t,
+// starting from the gradient of the final state and ending in the gradient of the initial one.
+//
+// What bounds it: two additions and two products a value against 6 to 14 bytes of memory; each kernel
+// reads and writes every array once.
+//
+// Split.  A workgroup of 8 wavefronts takes a tile of 8 S rows by 64 VEC channels; wavefront w holds S
+// consecutive rows of it in registers, a lane holds VEC neighbouring channels of each.  One pass over
+// the registers gives the wavefront's map, LDS combines the wavefronts, a second pass replays the rows
+// from the state that enters them and stores.  The rows of a sequence that span tiles are joined by
+// tile descriptors: every tile publishes its map, the 8th of a group of 8 tiles the map of the group,
+// the 64th of a super-group the state itself.  A tile reads at most one state, 7 group maps and 7 tile
+// maps and folds them in the order of the rows: what is combined with what depends on the sizes alone,
+// so results do not vary from run to run.
+//
+// Descriptors.  A map is one 64-bit word (A's bits << 32 | H's bits), stored inverted in a single
+// relaxed agent-scope atomic; NaNs are stored as the canonical one, so no map is the word 0, which
+// means "not there yet" and is what the clearing kernel leaves.
+//
+// Sequences.  A row that begins a sequence takes its initial state by selection, never by a product
+// with zero, so infinities and NaNs of one sequence stay in it.  Which predecessors a tile needs
+// follows from the offsets alone, as does whether a published map begins anew.
+#include <atomic>
+
+#include "lm_types.h"
+
+namespace tcd {
+
+constexpr int kLinWaves = 8;
+constexpr int kLinBlock = kLinWaves * kWave;
+constexpr int kLinGroup = 8;   // tiles of a group, groups of a super-group
+constexpr int kLinSuper = kLinGroup * kLinGroup;
+constexpr int kLinChunk = THRUST_CDNA4_LINEAR_SCAN_CHUNK;
+constexpr uint32_t kLinSpinLimit = 1u << 22;
+
+__device__ unsigned int g_linear_scan_timeouts;
+
+struct LinArgs {
+  const void* gate;
+  const void* x;
+  void* out;               // backward: grad_x
+  const void* grad_out;    // backward
+  void* grad_gate;         // backward
+  const float* init;
+  float* final_state;      // backward: grad_init
+  const float* grad_final; // backward
+  float* states;
+  const void* offsets;
+  int64_t gate_bs, gate_rs, x_bs, x_rs, out_bs, out_rs, grad_bs, grad_rs, grad_gate_bs, grad_gate_rs;
+  int64_t rows, channels;
+  int sequences, offsets64, log_gate, clear_outside;
+  int batch, ntiles, ncb;
+  uint32_t* ticket;
+  uint64_t* tile_map;   // [batch][ntiles][channels]
+  uint64_t* group_map;  // [batch][groups][channels]
+  uint32_t* super_state;  // [batch][super-groups][channels]
+};
+
+// ---------------------------------------------------------------------------------------
+// Published maps
+// ---------------------------------------------------------------------------------------
+__device__ inline uint32_t canonical_bits(float v) { return v != v ? 0x7fc00000u : bit_cast<uint32_t>(v); }
+
+__device__ inline void publish_map(uint64_t* p, float a, float h) {
+  st_agent(p, ~(((uint64_t)canonical_bits(a) << 32) | canonical_bits(h)));
+}
+
+// The ticket order makes every predecessor a running workgroup, so these waits end; the limit keeps a
+// mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts).
+template <int VEC, class W>
+__device__ inline void wait_words(const W* p, W (&v)[VEC]) {
+  for (uint32_t spins = 0;; spins++) {
+    bool all = true;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) v[j] = ld_agent(p + j);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) all = all && v[j] != 0;
+    if (all) break;
+    if (spins >= kLinSpinLimit) {
+      atomicAdd(&g_linear_scan_timeouts, 1u);
+      break;
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Sequences of packed rows.  Everything here is the same in all lanes of a wavefront.  Offsets that
+// do not ascend give meaningless results but no access outside the arrays.
+// ---------------------------------------------------------------------------------------
+__device__ inline int64_t offset_at(const LinArgs& p, int64_t j) {
+  return p.offsets64 ? static_cast<const int64_t*>(p.offsets)[j] : (int64_t) static_cast<const int32_t*>(p.offsets)[j];
+}
+
+// The last sequence that begins at or before `row` (not empty if `row` is inside one), or -1.  64 offsets a step.
+__device__ inline int sequence_of(const LinArgs& p, int64_t row) {
+  const int lane = lane_id();
+  int lo = 0, n = p.sequences + 1;  // the answer + 1 is the number of offsets <= row among lo .. lo + n - 1, plus lo
+  while (n > kWave) {
+    const int step = (n + kWave - 1) / kWave;
+    const int at = lane * step;
+    const bool below = at < n && offset_at(p, lo + at) <= row;
+    const int full = __popcll(__ballot(below));
+    if (full == 0) return lo - 1;
+    const int skip = (full - 1) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  const bool below = lane < n && offset_at(p, lo + lane) <= row;
+  return __builtin_amdgcn_readfirstlane(lo + __popcll(__ballot(below)) - 1);
+}
+
+// What a wavefront needs to know of its S rows: which of them are inside a sequence, begin one or end
+// one (bit k: row r0 + k), and the sequence of the first of them.
+struct RowSpan {
+  uint32_t inside, heads, ends;
+  int first_sequence;
+};
+
+template <int S, bool PACKED>
+__device__ inline RowSpan row_span(const LinArgs& p, int b, int64_t r0) {
+  RowSpan r{0, 0, 0, b};
+  const int64_t left = p.rows - r0;
+  const int n = left <= 0 ? 0 : left < S ? (int)left : S;
+  if (n == 0) return r;
+  const uint32_t all = (uint32_t)((uint64_t(1) << n) - 1);
+  if constexpr (!PACKED) {
+    r.inside = all;
+    r.heads = r0 == 0;
+    r.ends = left <= S ? 1u << (n - 1) : 0u;
+  } else {
+    const int64_t begin = offset_at(p, 0);
+    int64_t end = offset_at(p, p.sequences);
+    if (end > p.rows) end = p.rows;
+    const int64_t lo = begin > r0 ? begin - r0 : 0, hi = end - r0 < n ? end - r0 : n;
+    if (lo >= hi) return r;
+    r.inside = (uint32_t)((uint64_t(1) << hi) - 1) & ~(uint32_t)((uint64_t(1) << lo) - 1);
+    int s = sequence_of(p, r0 + lo);
+    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
+    r.first_sequence = s;
+    if (offset_at(p, s) == r0 + lo) r.heads |= 1u << lo;
+    for (int edges = 0; edges <= S; edges++) {  // each edge ends a sequence and, behind empty ones, begins another
+      const int64_t next = offset_at(p, s + 1);
+      if (next > r0 + hi || next <= r0) break;
+      r.ends |= 1u << (int)(next - r0 - 1);
+      const int after = next < r0 + hi ? sequence_of(p, next) : p.sequences;
+      if (after <= s || after >= p.sequences) break;
+      r.heads |= 1u << (int)(next - r0);
+      s = after;
+    }
+    r.heads &= r.inside;
+    r.ends &= r.inside;
+  }
+  return r;
+}
+template <bool PACKED>
+__device__ inline void next_sequence(const LinArgs& p, int64_t row, int& s) {  // to the one that `row` begins
+  if constexpr (PACKED) {
+    if (offset_at(p, s + 1) > row) return;
+    s = sequence_of(p, row);
+    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
+  }
+}
+template <bool PACKED>
+__device__ inline void previous_sequence(const LinArgs& p, int64_t row, int& s) {  // to the one that holds `row`
+  if constexpr (PACKED) {
+    if (offset_at(p, s) <= row) return;
+    s = sequence_of(p, row);
+    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
+  }
+}
+
+template <int VEC>
+__device__ inline void load_state(const float* p, int64_t at, float (&h)[VEC]) {
+  if (p) {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) h[j] = p[at + j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) h[j] = 0.f;
+  }
+}
+template <int VEC>
+__device__ inline void store_state(float* p, int64_t at, const float (&h)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; j++) p[at + j] = h[j];
+}
+
+// ---------------------------------------------------------------------------------------
+// The state that enters a tile.  "Logical" tiles and wavefronts are numbered in the direction of the
+// scan: as the rows for the recurrence, from the last one for its gradient.
+// ---------------------------------------------------------------------------------------
+template <int CH>
+struct LinShared {
+  float a[kLinWaves][CH], h[kLinWaves][CH];    // maps of the tile's wavefronts
+  float pa[kLinWaves][CH], ph[kLinWaves][CH];  // maps of earlier tiles, then of earlier groups
+  float state[CH];                             // state of the super-group before
+  float carry[CH];
+  int anew[kLinWaves];  // wavefront: a sequence begins in it (its h is then a state)
+  int64_t since;        // logical row in which the sequence of the tile's first row begins; -1: none comes in
+  uint32_t ticket;
+};
+
+// One channel: the maps m0, m0 + 1 .. m1 - 1 of (a, h) after (A, H)
+template <int CH>
+__device__ inline void fold(const float (*a)[CH], const float (*h)[CH], int m0, int m1, int ch, float& A, float& H) {
+  for (int m = m0; m < m1; m++) {
+    H = a[m][ch] * H + h[m][ch];
+    A *= a[m][ch];
+  }
+}
+
+// Called by the whole workgroup after sm.a, sm.h, sm.anew and sm.since are written and a barrier.
+// `i`: logical tile of `nt`; `rows`: rows of a tile.  Leaves the entering state in sm.carry.
+template <int VEC>
+__device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, int b, int64_t i, int64_t nt, int rows, int64_t c0, bool active,
+                                  int64_t block_c0) {
+  constexpr int CH = kWave * VEC;
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  const int64_t C = p.channels, groups = ceil_div(nt, kLinGroup), supers = ceil_div(nt, kLinSuper);
+  const bool publishes = i + 1 < nt;
+  const int64_t since = sm.since;
+  const bool needs = since >= 0;             // a sequence comes in from earlier tiles
+  const int64_t first = needs ? since / rows : i;  // the tile it begins in
+  const int64_t g = i / kLinGroup, base = g * kLinGroup, sg = g / kLinGroup;
+
+  int last_anew = -1;
+#pragma unroll
+  for (int v = 0; v < kLinWaves; v++)
+    if (sm.anew[v]) last_anew = v;
+  // the tile's own map for channel ch (a state, with A unused, where a sequence begins in it)
+  auto tile_total = [&](int ch, float& A, float& H) {
+    A = 1.f;
+    H = last_anew >= 0 ? sm.h[last_anew][ch] : 0.f;
+    fold<CH>(sm.a, sm.h, last_anew + 1, kLinWaves, ch, A, H);
+  };
+  // the last wavefront publishes the tile's map, the others wait for those of the group
+  if (w == kLinWaves - 1) {
+    if (publishes && active) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        float A, H;
+        tile_total(lane * VEC + j, A, H);
+        publish_map(p.tile_map + ((int64_t)b * nt + i) * C + c0 + j, A, H);
+      }
+    }
+  } else if (needs && base + w < i && base + w >= first && active) {
+    uint64_t v[VEC];
+    wait_words<VEC>(p.tile_map + ((int64_t)b * nt + base + w) * C + c0, v);
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      sm.pa[w][lane * VEC + j] = bit_cast<float>((uint32_t)(~v[j] >> 32));
+      sm.ph[w][lane * VEC + j] = bit_cast<float>((uint32_t)~v[j]);
+    }
+  }
+  __syncthreads();
+  // a thread for each channel from here on; (GA, GH) is the map of the group's earlier tiles, or GH a state
+  const int ch = tid;
+  const int64_t chan = [&] {
+    const int64_t at = block_c0 + ch / VEC * VEC;
+    return (at + VEC > C ? C - VEC : at) + ch % VEC;
+  }();
+  const bool mine = ch < CH && block_c0 + ch / VEC * VEC < C;
+  const bool in_group = needs && first >= base;
+  float GA = 1.f, GH = 0.f;
+  if (mine) {
+    if (in_group && i > base) {
+      GH = sm.ph[first - base][ch];
+      fold<CH>(sm.pa, sm.ph, (int)(first - base) + 1, (int)(i - base), ch, GA, GH);
+    } else if (needs) {
+      fold<CH>(sm.pa, sm.ph, 0, (int)(i - base), ch, GA, GH);
+    }
+    if (publishes && i - base == kLinGroup - 1) {
+      float A, H;
+      tile_total(ch, A, H);
+      if (last_anew < 0) {
+        H = A * GH + H;
+        A *= GA;
+      }
+      publish_map(p.group_map + ((int64_t)b * groups + g) * C + chan, A, H);
+    }
+  }
+  if (needs && !in_group) {
+    __syncthreads();  // pa and ph are free again
+    const int64_t gbase = sg * kLinGroup, gfirst = first / kLinGroup;
+    if (w == kLinWaves - 1) {
+      if (gfirst < gbase && active) {
+        uint32_t v[VEC];
+        wait_words<VEC>(p.super_state + ((int64_t)b * supers + sg - 1) * C + c0, v);
+#pragma unroll
+        for (int j = 0; j < VEC; j++) sm.state[lane * VEC + j] = bit_cast<float>(~v[j]);
+      }
+    } else if (gbase + w < g && gbase + w >= gfirst && active) {
+      uint64_t v[VEC];
+      wait_words<VEC>(p.group_map + ((int64_t)b * groups + gbase + w) * C + c0, v);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        sm.pa[w][lane * VEC + j] = bit_cast<float>((uint32_t)(~v[j] >> 32));
+        sm.ph[w][lane * VEC + j] = bit_cast<float>((uint32_t)~v[j]);
+      }
+    }
+    __syncthreads();
+    if (mine) {
+      float A = 1.f, H;
+      int from = 0;
+      if (gfirst < gbase) H = sm.state[ch];
+      else H = sm.ph[gfirst - gbase][ch], from = (int)(gfirst - gbase) + 1;
+      fold<CH>(sm.pa, sm.ph, from, (int)(g - gbase), ch, A, H);
+      GH = GA * H + GH;
+    }
+  }
+  if (mine) {
+    sm.carry[ch] = GH;
+    if (publishes && i % kLinSuper == kLinSuper - 1) {
+      float A, H;
+      tile_total(ch, A, H);
+      if (last_anew < 0) H = A * GH + H;
+      st_agent(p.super_state + ((int64_t)b * supers + sg) * C + chan, ~canonical_bits(H));
+    }
+  }
+  __syncthreads();
+}
+
+// The state that enters logical wavefront `lw` of the tile
+template <int VEC>
+__device__ inline void wave_carry(const LinShared<kWave * VEC>& sm, int lw, int lane, float (&h)[VEC]) {
+  int last_anew = -1;
+  for (int v = 0; v < lw; v++)
+    if (sm.anew[v]) last_anew = v;
+#pragma unroll
+  for (int j = 0; j < VEC; j++) {
+    const int ch = lane * VEC + j;
+    float A = 1.f;
+    h[j] = last_anew >= 0 ? sm.h[last_anew][ch] : sm.carry[ch];
+    fold<kWave * VEC>(sm.a, sm.h, last_anew + 1, lw, ch, A, h[j]);
+  }
+}
+
+// Which tile this workgroup takes: in the order of a ticket where tiles wait for one another (a tile
+// then only waits for running ones), by its index where none does.
+__device__ inline void take_lin_tile(const LinArgs& p, uint32_t* shared, int64_t& i, int& b, int& cb) {
+  uint32_t t = blockIdx.x;
+  if (p.ticket) {
+    if (threadIdx.x == 0) *shared = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    t = *shared;
+  }
+  const uint32_t across = (uint32_t)p.batch * (uint32_t)p.ncb;
+  i = t / across;
+  const uint32_t rest = t % across;
+  cb = (int)(rest % (uint32_t)p.ncb);
+  b = (int)(rest / (uint32_t)p.ncb);
+}
+
+// States of sequences without rows: the final state is the initial one (the gradients likewise).
+template <int VEC>
+__device__ inline void empty_sequences(const LinArgs& p, int64_t i, const float* from, float* to, int64_t c0, bool active) {
+  const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  for (int64_t s0 = (i * kLinWaves + w) * kWave; s0 < p.sequences; s0 += (int64_t)p.ntiles * kLinWaves * kWave) {
+    const int64_t s = s0 + lane;
+    uint64_t none = __ballot(s < p.sequences && offset_at(p, s) >= offset_at(p, s + 1));
+    while (none) {
+      const int64_t at = (s0 + __builtin_ctzll(none)) * p.channels + c0;
+      none &= none - 1;
+      float h[VEC];
+      load_state<VEC>(from, at, h);
+      if (active) store_state<VEC>(to, at, h);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// The recurrence
+// ---------------------------------------------------------------------------------------
+template <class TG, class TX, int VEC, int S, bool PACKED>
+__global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
+  constexpr int CH = kWave * VEC, R = S * kLinWaves;
+  __shared__ LinShared<CH> sm;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  int64_t i;
+  int b, cb;
+  take_lin_tile(p, &sm.ticket, i, b, cb);
+  const int64_t C = p.channels, block_c0 = (int64_t)cb * CH;
+  // the last lane's vector ends with the last channel: it may repeat channels of the lane before it,
+  // and stores the same values
+  const int64_t at = block_c0 + lane * VEC;
+  const bool active = at < C;
+  const int64_t c0 = at + VEC > C ? C - VEC : at;
+  const int64_t r0 = i * R + w * S;
+  const int64_t left = p.rows - r0;
+
+  Pack<TG, VEC> gate[S];
+  Pack<TX, VEC> x[S];
+  if (left > 0) {
+    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + c0;
+    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + c0;
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      const int64_t row = k < left ? r0 + k : p.rows - 1;
+      gate[k] = load_pack<TG, VEC>(gp + row * p.gate_rs);
+      x[k] = load_pack<TX, VEC>(xp + row * p.x_rs);
+    }
+  }
+  const RowSpan span = row_span<S, PACKED>(p, b, r0);
+  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return p.log_gate ? expf(g.value(j)) : g.value(j); };
+  auto step = [&](int k, float (&h)[VEC], float (&A)[VEC], int& s) {
+    if (span.heads >> k & 1) {
+      next_sequence<PACKED>(p, r0 + k, s);
+      load_state<VEC>(p.init, (int64_t)s * C + c0, h);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      const float a = gate_value(gate[k], j);
+      h[j] = a * h[j] + x[k].value(j);
+      A[j] *= a;
+    }
+  };
+  float h[VEC], A[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = 1.f;
+  int s = span.first_sequence;
+#pragma unroll
+  for (int k = 0; k < S; k++)
+    if (span.inside >> k & 1) step(k, h, A, s);
+#pragma unroll
+  for (int j = 0; j < VEC; j++) {
+    sm.a[w][lane * VEC + j] = A[j];
+    sm.h[w][lane * VEC + j] = h[j];
+  }
+  if (lane == 0) sm.anew[w] = span.heads != 0;
+  if (w == 0) {
+    int64_t since = -1;
+    if (!(span.heads & 1) && (span.inside & 1)) since = PACKED ? offset_at(p, span.first_sequence) : 0;
+    if (lane == 0) sm.since = since < 0 || since > r0 ? -1 : since;
+  }
+  __syncthreads();
+  if (p.ntiles > 1) {
+    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, c0, active, block_c0);
+  } else {
+    if (tid < CH) sm.carry[tid] = 0.f;
+    __syncthreads();
+  }
+
+  wave_carry<VEC>(sm, w, lane, h);
+  s = span.first_sequence;
+  if (p.states && left > 0 && r0 % kLinChunk == 0 && active) {
+    if (span.heads & 1) load_state<VEC>(p.init, (int64_t)s * C + c0, A);
+    store_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + r0 / kLinChunk) * C + c0, span.heads & 1 ? A : h);
+  }
+  TX* out = static_cast<TX*>(p.out) + b * p.out_bs + c0;
+#pragma unroll
+  for (int k = 0; k < S; k++) forget(gate[k]), forget(x[k]);
+#pragma unroll
+  for (int k = 0; k < S; k++) {
+    if (span.inside >> k & 1) {
+      step(k, h, A, s);
+      if (active) {
+        store_pack<TX, VEC>(out + (r0 + k) * p.out_rs, Pack<TX, VEC>::of(h));
+        if (p.final_state && span.ends >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C + c0, h);
+      }
+    } else if (PACKED && p.clear_outside && k < left && active) {
+      store_pack<TX, VEC>(out + (r0 + k) * p.out_rs, Pack<TX, VEC>{});
+    }
+  }
+  if (p.final_state) {
+    if constexpr (PACKED) {
+      empty_sequences<VEC>(p, i, p.init, p.final_state, c0, active);
+    } else if (p.rows == 0 && w == 0) {
+      load_state<VEC>(p.init, (int64_t)b * C + c0, h);
+      if (active) store_state<VEC>(p.final_state, (int64_t)b * C + c0, h);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Its gradient.  A tile is one chunk: the state that enters it was kept by the recurrence, so the
+// states of its rows are computed again, in 32 bits, from the gates and inputs, which costs no more
+// memory traffic than reading the outputs would and does not differentiate their rounding.
+// ---------------------------------------------------------------------------------------
+template <class TG, class TX, int VEC, bool PACKED>
+__global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs p) {
+  constexpr int S = kLinChunk / kLinWaves, CH = kWave * VEC, R = kLinChunk;
+  __shared__ LinShared<CH> sm;
+  __shared__ float fwd[kLinWaves][CH];
+  __shared__ int fwd_anew[kLinWaves];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int lw = kLinWaves - 1 - w;
+  int64_t i;  // from the last tile
+  int b, cb;
+  take_lin_tile(p, &sm.ticket, i, b, cb);
+  const int64_t tile = p.ntiles - 1 - i;
+  const int64_t C = p.channels, block_c0 = (int64_t)cb * CH;
+  const int64_t at = block_c0 + lane * VEC;
+  const bool active = at < C;
+  const int64_t c0 = at + VEC > C ? C - VEC : at;
+  const int64_t r0 = tile * R + w * S;
+  const int64_t left = p.rows - r0;
+
+  Pack<TG, VEC> gate[S];
+  Pack<TX, VEC> x[S], d[S];
+  float h[VEC], enter[VEC];
+  if (left > 0) {
+    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + c0;
+    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + c0;
+    const TX* dp = static_cast<const TX*>(p.grad_out) + b * p.grad_bs + c0;
+#pragma unroll
+    for (int k = 0; k < S; k++) {
+      const int64_t row = k < left ? r0 + k : p.rows - 1;
+      gate[k] = load_pack<TG, VEC>(gp + row * p.gate_rs);
+      x[k] = load_pack<TX, VEC>(xp + row * p.x_rs);
+      d[k] = load_pack<TX, VEC>(dp + row * p.grad_rs);
+    }
+    load_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + tile) * C + c0, enter);
+  }
+  const RowSpan span = row_span<S, PACKED>(p, b, r0);
+  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return p.log_gate ? expf(g.value(j)) : g.value(j); };
+  // one row of the recurrence, and one of its gradient (c: in the gradient of the state after the row, out that of the one before)
+  auto step = [&](int k, float (&hh)[VEC], int& s) {
+    if (span.heads >> k & 1) {
+      next_sequence<PACKED>(p, r0 + k, s);
+      load_state<VEC>(p.init, (int64_t)s * C + c0, hh);
+    }
+  };
+  auto turn = [&](int k, float (&c)[VEC], int& s) {
+    if (span.ends >> k & 1) {
+      previous_sequence<PACKED>(p, r0 + k, s);
+      load_state<VEC>(p.grad_final, (int64_t)s * C + c0, c);
+    }
+  };
+  float A[VEC], c[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = 1.f, c[j] = 0.f;
+  int s = span.first_sequence;
+#pragma unroll
+  for (int k = 0; k < S; k++) {
+    if (span.inside >> k & 1) {
+      step(k, h, s);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        const float a = gate_value(gate[k], j);
+        h[j] = a * h[j] + x[k].value(j);
+        A[j] *= a;
+      }
+    }
+  }
+  const int last_sequence = s;
+#pragma unroll
+  for (int k = S - 1; k >= 0; k--) {
+    if (span.inside >> k & 1) {
+      turn(k, c, s);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) c[j] = gate_value(gate[k], j) * (d[k].value(j) + c[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; j++) {
+    sm.a[lw][lane * VEC + j] = A[j];
+    sm.h[lw][lane * VEC + j] = c[j];
+    fwd[w][lane * VEC + j] = h[j];
+  }
+  if (lane == 0) {
+    sm.anew[lw] = span.ends != 0;
+    fwd_anew[w] = span.heads != 0;
+  }
+  // the sequence of the tile's last row: in how many logical rows before this tile it begins (that is, ends)
+  if (w == kLinWaves - 1) {
+    int64_t since = -1;
+    const int64_t logical = (int64_t)p.ntiles * R - 1;
+    if (!(span.ends >> (S - 1) & 1) && (span.inside >> (S - 1) & 1)) {
+      int64_t end = p.rows;
+      if constexpr (PACKED) end = offset_at(p, last_sequence + 1);
+      since = end > p.rows ? -1 : logical - (end - 1);
+    }
+    if (lane == 0) sm.since = since < 0 || since >= i * R ? -1 : since;
+  }
+  __syncthreads();
+  if (p.ntiles > 1) {
+    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, c0, active, block_c0);
+  } else {
+    if (tid < CH) sm.carry[tid] = 0.f;
+    __syncthreads();
+  }
+
+  // states before each row
+  int last_anew = -1;
+  for (int v = 0; v < w; v++)
+    if (fwd_anew[v]) last_anew = v;
+  if (left > 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      const int ch = lane * VEC + j;
+      h[j] = last_anew >= 0 ? fwd[last_anew][ch] : enter[j];
+      for (int v = last_anew + 1; v < w; v++) h[j] = sm.a[kLinWaves - 1 - v][ch] * h[j] + fwd[v][ch];
+    }
+  }
+  float before[S][VEC];
+  s = span.first_sequence;
+#pragma unroll
+  for (int k = 0; k < S; k++) {
+    if (span.inside >> k & 1) {
+      step(k, h, s);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        before[k][j] = h[j];
+        h[j] = gate_value(gate[k], j) * h[j] + x[k].value(j);
+      }
+    }
+  }
+  wave_carry<VEC>(sm, lw, lane, c);
+  TG* grad_gate = static_cast<TG*>(p.grad_gate) + b * p.grad_gate_bs + c0;
+  TX* grad_x = static_cast<TX*>(p.out) + b * p.out_bs + c0;
+#pragma unroll
+  for (int k = S - 1; k >= 0; k--) {
+    if (span.inside >> k & 1) {
+      turn(k, c, s);
+      previous_sequence<PACKED>(p, r0 + k, s);
+      float dg[VEC], dx[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        const float a = gate_value(gate[k], j);
+        const float g = d[k].value(j) + c[j];
+        const float da = g * before[k][j];
+        c[j] = a * g;
+        dx[j] = g;
+        dg[j] = p.log_gate ? da * a : da;
+      }
+      if (active) {
+        store_pack<TX, VEC>(grad_x + (r0 + k) * p.out_rs, Pack<TX, VEC>::of(dx));
+        store_pack<TG, VEC>(grad_gate + (r0 + k) * p.grad_gate_rs, Pack<TG, VEC>::of(dg));
+        if (p.final_state && span.heads >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C + c0, c);
+      }
+    } else if (PACKED && p.clear_outside && k < left && active) {
+      store_pack<TX, VEC>(grad_x + (r0 + k) * p.out_rs, Pack<TX, VEC>{});
+      store_pack<TG, VEC>(grad_gate + (r0 + k) * p.grad_gate_rs, Pack<TG, VEC>{});
+    }
+  }
+  if (p.final_state) {
+    if constexpr (PACKED) {
+      empty_sequences<VEC>(p, i, p.grad_final, p.final_state, c0, active);
+    } else if (p.rows == 0 && w == 0) {
+      load_state<VEC>(p.grad_final, (int64_t)b * C + c0, h);
+      if (active) store_state<VEC>(p.final_state, (int64_t)b * C + c0, h);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// One token for each of a batch: state[slot] = a state[slot] + x, out = state.  Rows of one slot are
+// taken in their order: the first of them does all, the others leave.
+// ---------------------------------------------------------------------------------------
+constexpr int kStepBlock = 256;
+
+template <class TG, class TX, int VEC>
+__global__ __launch_bounds__(kStepBlock) void linear_scan_step_kernel(const TG* gate, int64_t gate_rs, const TX* x, int64_t x_rs, TX* out,
+                                                                      int64_t out_rs, float* state, int64_t num_slots, const int32_t* slots,
+                                                                      int batch, int64_t C, int ncb, int log_gate) {
+  __shared__ int s_earlier, s_later;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int row = (int)(blockIdx.x / (unsigned)ncb), cb = (int)(blockIdx.x % (unsigned)ncb);
+  const int64_t at = ((int64_t)cb * kStepBlock + tid) * VEC;
+  const bool active = at < C;
+  const int64_t c0 = at + VEC > C ? C - VEC : at;
+  const int64_t slot = slots ? slots[row] : row;
+  if (slot < 0 || slot >= num_slots) {  // a padded row
+    if (active) store_pack<TX, VEC>(out + row * out_rs + c0, Pack<TX, VEC>{});
+    return;
+  }
+  Pack<TG, VEC> g = load_pack<TG, VEC>(gate + row * gate_rs + c0);
+  Pack<TX, VEC> v = load_pack<TX, VEC>(x + row * x_rs + c0);
+  float* sp = state + slot * C + c0;
+  float h[VEC];
+  load_state<VEC>(sp, 0, h);
+  if (slots) {
+    if (tid < kWave) {
+      uint64_t earlier = 0, later = 0;
+      for (int q = lane; q < batch + lane; q += kWave) {
+        const bool same = q < batch && slots[q < batch ? q : batch - 1] == slot;
+        earlier |= __ballot(same && q < row);
+        later |= __ballot(same && q > row);
+      }
+      if (tid == 0) s_earlier = earlier != 0, s_later = later != 0;
+    }
+    __syncthreads();
+    if (s_earlier) return;
+  }
+  auto one = [&](int q) {
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      const float a = log_gate ? expf(g.value(j)) : g.value(j);
+      h[j] = a * h[j] + v.value(j);
+    }
+    if (active) store_pack<TX, VEC>(out + q * out_rs + c0, Pack<TX, VEC>::of(h));
+  };
+  one(row);
+  if (slots && s_later) {
+    for (int q = row + 1; q < batch; q++) {
+      if (slots[q] != slot) continue;
+      g = load_pack<TG, VEC>(gate + q * gate_rs + c0);
+      v = load_pack<TX, VEC>(x + q * x_rs + c0);
+      one(q);
+    }
+  }
+  if (active) store_state<VEC>(sp, 0, h);
+}
+
+// ---------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------
+// (gate, x) types: the same, or 32-bit gates with 16-bit inputs
+template <class F>
+inline bool dispatch_activation(int gate, int x, F&& f) {
+  if (gate == THRUST_CDNA4_F32 && x == THRUST_CDNA4_F32) return f(float{}, float{}), true;
+  if (gate == THRUST_CDNA4_F16 && x == THRUST_CDNA4_F16) return f(f16_t{}, f16_t{}), true;
+  if (gate == THRUST_CDNA4_BF16 && x == THRUST_CDNA4_BF16) return f(bf16_t{}, bf16_t{}), true;
+  if (gate == THRUST_CDNA4_F32 && x == THRUST_CDNA4_F16) return f(float{}, f16_t{}), true;
+  if (gate == THRUST_CDNA4_F32 && x == THRUST_CDNA4_BF16) return f(float{}, bf16_t{}), true;
+  return false;
+}
+
+struct LinPlan {
+  int vec, ncb;
+  int64_t ntiles;
+  size_t tile_at, group_at, super_at, bytes, clear;
+};
+
+inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_rows, bool narrow, LinPlan& l) {
+  l.vec = narrow ? 1 : 4;
+  const int64_t ncb = ceil_div(channels, (int64_t)kWave * l.vec);
+  l.ntiles = rows > 0 ? ceil_div(rows, (int64_t)tile_rows) : 1;
+  const double grid = (double)ncb * (double)batch * (double)l.ntiles;
+  if (grid > 2147483647.0) return false;
+  l.ncb = (int)ncb;
+  l.bytes = 256;
+  l.clear = 0;
+  if (l.ntiles > 1) {
+    const size_t across = (size_t)batch * (size_t)channels;
+    l.tile_at = 256;
+    l.group_at = l.tile_at + align_up(across * (size_t)l.ntiles * 8, 256);
+    l.super_at = l.group_at + align_up(across * (size_t)ceil_div(l.ntiles, (int64_t)kLinGroup) * 8, 256);
+    l.bytes = l.super_at + align_up(across * (size_t)ceil_div(l.ntiles, (int64_t)kLinSuper) * 4, 256);
+    l.clear = l.bytes;
+  }
+  return true;
+}
+
+inline void lin_storage(LinArgs& p, const LinPlan& l, void* temp) {
+  p.ntiles = (int)l.ntiles;
+  p.ncb = l.ncb;
+  p.ticket = nullptr;
+  if (l.ntiles > 1) {
+    char* t = static_cast<char*>(temp);
+    p.ticket = reinterpret_cast<uint32_t*>(t);
+    p.tile_map = reinterpret_cast<uint64_t*>(t + l.tile_at);
+    p.group_map = reinterpret_cast<uint64_t*>(t + l.group_at);
+    p.super_state = reinterpret_cast<uint32_t*>(t + l.super_at);
+  }
+}
+
+// rows of the recurrence's tile: the payload of a lane is 64 registers at most
+template <class TG, class TX>
+constexpr int lin_rows_per_wave() { return sizeof(TG) == 2 && sizeof(TX) == 2 ? 16 : 8; }
+
+inline bool valid_shape(int64_t batch, int64_t rows, int64_t channels, int64_t sequences, const void* offsets, int offset_bytes) {
+  if (batch < 0 || rows < 0 || channels < 0 || channels > 0x7fffffff || batch > 0x7fffffff) return false;
+  if (offsets || offset_bytes) return batch == 1 && (offset_bytes == 4 || offset_bytes == 8) && sequences >= 0 && sequences < 0x7fffffff;
+  return true;
+}
+
+// the bytes that rows of this shape and these strides span (strides are not negative)
+inline size_t span_bytes(int64_t batch, int64_t rows, int64_t channels, int64_t bs, int64_t rs, int elem) {
+  if (batch == 0 || rows == 0 || channels == 0) return 0;
+  return (size_t)((batch - 1) * bs + (rows - 1) * rs + channels) * (size_t)elem;
+}
+
+// Four channels a lane where half of a wavefront's lanes find work, one otherwise.  An output over an
+// input allows the former only where no vector reaches over a workgroup's channels.
+inline bool lin_narrow(int64_t channels, bool in_place) { return channels <= 128 || (in_place && channels % 4 != 0); }
+
+}  // namespace tcd
+
+extern "C" int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const thrust_cdna4_linear_scan_args* a, void* stream) {
+  using namespace tcd;
+  if (!temp_bytes || !a || temp_misaligned(temp)) return hipErrorInvalidValue;
+  const bool packed = a->offset_bytes != 0;
+  if (!valid_shape(a->batch, a->rows, a->channels, a->sequences, a->offsets, a->offset_bytes)) return hipErrorInvalidValue;
+  if (!activation_size(a->gate_dtype) || !activation_size(a->x_dtype)) return hipErrorInvalidValue;
+  const size_t span_x = span_bytes(a->batch, a->rows, a->channels, a->x_batch_stride, a->x_row_stride, activation_size(a->x_dtype));
+  const size_t span_g = span_bytes(a->batch, a->rows, a->channels, a->gate_batch_stride, a->gate_row_stride, activation_size(a->gate_dtype));
+  const size_t span_o = span_bytes(a->batch, a->rows, a->channels, a->out_batch_stride, a->out_row_stride, activation_size(a->x_dtype));
+  const bool in_place = a->out && (ranges_overlap(a->out, span_o, a->x, span_x) || ranges_overlap(a->out, span_o, a->gate, span_g));
+  hipError_t rc = hipErrorInvalidValue;
+  dispatch_activation(a->gate_dtype, a->x_dtype, [&](auto tg, auto tx) {
+    using TG = decltype(tg);
+    using TX = decltype(tx);
+    constexpr int S = lin_rows_per_wave<TG, TX>();
+    LinPlan l;
+    const bool narrow = lin_narrow(a->channels, in_place);
+    if (!lin_plan(a->batch, a->rows, a->channels, S * kLinWaves, narrow, l)) return;
+    if (temp == nullptr) {
+      *temp_bytes = l.bytes;
+      rc = hipSuccess;
+      return;
+    }
+    const int64_t states = packed ? a->sequences : a->batch;
+    if (a->channels == 0 || a->batch == 0) {
+      rc = hipSuccess;
+      return;
+    }
+    if (*temp_bytes < l.bytes || (packed && !a->offsets)) return;
+    if (a->rows > 0 && (!a->gate || !a->x || !a->out)) return;
+    const size_t state_bytes = (size_t)states * (size_t)a->channels * 4;
+    if (a->init && a->final_state && ranges_overlap(a->init, state_bytes, a->final_state, state_bytes)) return;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LinArgs p{};
+    p.gate = a->gate, p.x = a->x, p.out = a->out;
+    p.init = static_cast<const float*>(a->init);
+    p.final_state = static_cast<float*>(a->final_state);
+    p.states = static_cast<float*>(a->states);
+    p.offsets = a->offsets, p.offsets64 = a->offset_bytes == 8, p.sequences = (int)a->sequences;
+    p.gate_bs = a->gate_batch_stride, p.gate_rs = a->gate_row_stride;
+    p.x_bs = a->x_batch_stride, p.x_rs = a->x_row_stride;
+    p.out_bs = a->out_batch_stride, p.out_rs = a->out_row_stride;
+    p.rows = a->rows, p.channels = a->channels, p.batch = (int)a->batch, p.log_gate = a->log_gate != 0, p.clear_outside = packed && a->clear_outside;
+    lin_storage(p, l, temp);
+    if (l.clear) {
+      rc = zero_async(temp, l.clear, s);
+      if (rc != hipSuccess) return;
+    }
+    const dim3 grid((unsigned)((int64_t)l.ncb * a->batch * l.ntiles));
+    auto go = [&](auto vec, auto pk) {
+      TCD_LAUNCH("linear_scan_kernel", (linear_scan_kernel<TG, TX, decltype(vec)::value, S, decltype(pk)::value>), grid, dim3(kLinBlock), s, p);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    if (l.vec == 1) packed ? go(One{}, std::true_type{}) : go(One{}, std::false_type{});
+    else packed ? go(Four{}, std::true_type{}) : go(Four{}, std::false_type{});
+    rc = hipGetLastError();
+  });
+  return (int)rc;
+}
+
+extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes, const thrust_cdna4_linear_scan_backward_args* a, void* stream) {
+  using namespace tcd;
+  if (!temp_bytes || !a || temp_misaligned(temp)) return hipErrorInvalidValue;
+  const bool packed = a->offset_bytes != 0;
+  if (!valid_shape(a->batch, a->rows, a->channels, a->sequences, a->offsets, a->offset_bytes)) return hipErrorInvalidValue;
+  if (!activation_size(a->gate_dtype) || !activation_size(a->x_dtype)) return hipErrorInvalidValue;
+  const int ex = activation_size(a->x_dtype), eg = activation_size(a->gate_dtype);
+  const size_t in_span[3] = {span_bytes(a->batch, a->rows, a->channels, a->x_batch_stride, a->x_row_stride, ex),
+                             span_bytes(a->batch, a->rows, a->channels, a->gate_batch_stride, a->gate_row_stride, eg),
+                             span_bytes(a->batch, a->rows, a->channels, a->grad_out_batch_stride, a->grad_out_row_stride, ex)};
+  const void* in_at[3] = {a->x, a->gate, a->grad_out};
+  const size_t span_dx = span_bytes(a->batch, a->rows, a->channels, a->grad_x_batch_stride, a->grad_x_row_stride, ex);
+  const size_t span_dg = span_bytes(a->batch, a->rows, a->channels, a->grad_gate_batch_stride, a->grad_gate_row_stride, eg);
+  bool in_place = false;
+  for (int k = 0; k < 3; k++)
+    in_place = in_place || (a->grad_x && ranges_overlap(a->grad_x, span_dx, in_at[k], in_span[k])) ||
+               (a->grad_gate && ranges_overlap(a->grad_gate, span_dg, in_at[k], in_span[k]));
+  hipError_t rc = hipErrorInvalidValue;
+  dispatch_activation(a->gate_dtype, a->x_dtype, [&](auto tg, auto tx) {
+    using TG = decltype(tg);
+    using TX = decltype(tx);
+    LinPlan l;
+    const bool narrow = lin_narrow(a->channels, in_place);
+    if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, narrow, l)) return;
+    if (temp == nullptr) {
+      *temp_bytes = l.bytes;
+      rc = hipSuccess;
+      return;
+    }
+    const int64_t states = packed ? a->sequences : a->batch;
+    if (a->channels == 0 || a->batch == 0) {
+      rc = hipSuccess;
+      return;
+    }
+    if (*temp_bytes < l.bytes || (packed && !a->offsets)) return;
+    if (a->rows > 0 && (!a->gate || !a->x || !a->grad_out || !a->grad_x || !a->grad_gate || !a->states)) return;
+    const size_t state_bytes = (size_t)states * (size_t)a->channels * 4;
+    if (a->grad_init && ((a->grad_final && ranges_overlap(a->grad_init, state_bytes, a->grad_final, state_bytes)) ||
+                         (a->init && ranges_overlap(a->grad_init, state_bytes, a->init, state_bytes))))
+      return;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    LinArgs p{};
+    p.gate = a->gate, p.x = a->x, p.grad_out = a->grad_out, p.out = a->grad_x, p.grad_gate = a->grad_gate;
+    p.init = static_cast<const float*>(a->init);
+    p.grad_final = static_cast<const float*>(a->grad_final);
+    p.final_state = static_cast<float*>(a->grad_init);
+    p.states = const_cast<float*>(static_cast<const float*>(a->states));
+    p.offsets = a->offsets, p.offsets64 = a->offset_bytes == 8, p.sequences = (int)a->sequences;
+    p.gate_bs = a->gate_batch_stride, p.gate_rs = a->gate_row_stride;
+    p.x_bs = a->x_batch_stride, p.x_rs = a->x_row_stride;
+    p.out_bs = a->grad_x_batch_stride, p.out_rs = a->grad_x_row_stride;
+    p.grad_bs = a->grad_out_batch_stride, p.grad_rs = a->grad_out_row_stride;
+    p.grad_gate_bs = a->grad_gate_batch_stride, p.grad_gate_rs = a->grad_gate_row_stride;
+    p.rows = a->rows, p.channels = a->channels, p.batch = (int)a->batch, p.log_gate = a->log_gate != 0, p.clear_outside = packed && a->clear_outside;
+    lin_storage(p, l, temp);
+    if (l.clear) {
+      rc = zero_async(temp, l.clear, s);
+      if (rc != hipSuccess) return;
+    }
+    const dim3 grid((unsigned)((int64_t)l.ncb * a->batch * l.ntiles));
+    auto go = [&](auto vec, auto pk) {
+      TCD_LAUNCH("linear_scan_backward_kernel", (linear_scan_backward_kernel<TG, TX, decltype(vec)::value, decltype(pk)::value>), grid,
+                 dim3(kLinBlock), s, p);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    if (l.vec == 1) packed ? go(One{}, std::true_type{}) : go(One{}, std::false_type{});
+    else packed ? go(Four{}, std::true_type{}) : go(Four{}, std::false_type{});
+    rc = hipGetLastError();
+  });
+  return (int)rc;
+}
+
+extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, const void* gate, int64_t gate_row_stride,
+                                             const void* x, int64_t x_row_stride, void* out, int64_t out_row_stride, void* state,
+                                             int64_t num_slots, const int32_t* slots, int64_t batch, int64_t channels, void* stream) {
+  using namespace tcd;
+  if (batch < 0 || channels < 0 || num_slots < 0 || batch > 0x7fffffff || channels > 0x7fffffff) return hipErrorInvalidValue;
+  if (!activation_size(gate_dtype) || !activation_size(x_dtype)) return hipErrorInvalidValue;
+  if (!slots && batch > num_slots) return hipErrorInvalidValue;
+  hipError_t rc = hipErrorInvalidValue;
+  dispatch_activation(gate_dtype, x_dtype, [&](auto tg, auto tx) {
+    using TG = decltype(tg);
+    using TX = decltype(tx);
+    if (batch == 0 || channels == 0) {
+      rc = hipSuccess;
+      return;
+    }
+    if (!gate || !x || !out || (!state && num_slots > 0)) return;
+    // a vector that repeats channels of its neighbour would read a state that the neighbour has replaced
+    const int vec = channels % 4 != 0 ? 1 : 4;
+    const int64_t ncb = ceil_div(channels, (int64_t)kStepBlock * vec);
+    if ((double)ncb * (double)batch > 2147483647.0) return;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)(ncb * batch));
+    auto go = [&](auto v) {
+      TCD_LAUNCH("linear_scan_step_kernel", (linear_scan_step_kernel<TG, TX, decltype(v)::value>), grid, dim3(kStepBlock), s,
+                 static_cast<const TG*>(gate), gate_row_stride, static_cast<const TX*>(x), x_row_stride, static_cast<TX*>(out), out_row_stride,
+                 static_cast<float*>(state), num_slots, slots, (int)batch, channels, (int)ncb, log_gate != 0);
+    };
+    if (vec == 1) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 4>{});
+    rc = hipGetLastError();
+  });
+  return (int)rc;
+}
+
+namespace tcd {
+// waits of this file's kernels that did not end, on the current device
+hipError_t linear_scan_timeouts(unsigned int* count) {
+  return hipMemcpyFromSymbol(count, HIP_SYMBOL(g_linear_scan_timeouts), sizeof(*count));
+}
+}  // namespace tcd

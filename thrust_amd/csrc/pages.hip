@@ -1,0 +1,517 @@
+// Pages of a cache for gfx950: forking, growing, shrinking and freeing sequences, and compaction.
+//
+// Which pages are free is kept in one place, the counts (0: free), so a call begins by compacting the
+// indices of free pages: the counts are tallied in spans, a second launch adds up the spans before
+// its own and writes the indices in ascending order, as far as they are wanted.  Requests are served
+// by a prefix sum over what they want; request i takes free pages start[i] .. start[i] + need[i] - 1.
+// Nothing depends on the order in which workgroups run.
+//
+// What bounds it: with data to move, memory (each byte read and written once); without, the launches
+// (two or three small ones) and the 4 bytes of every count.
+#include "lm_types.h"
+
+namespace tcd {
+
+constexpr int kPageBlock = 256;
+constexpr int kPagesPerThread = 8;
+constexpr int kPageSweep = kPageBlock * kPagesPerThread;  // counts that a workgroup looks at in one go
+constexpr int kCopyUnit = kPageBlock * 16 * 4;            // bytes that a workgroup copies in one go
+constexpr int kMaxSpans = 8192;
+constexpr int kRequestWaves = kPageBlock / kWave;
+
+struct PageCache {
+  const uint64_t* pools;
+  int64_t page_bytes;
+  int num_pools, num_pages, page_size, num_sequences, max_pages;
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* refs;
+};
+
+// the temporary storage of a call
+struct PageTemp {
+  int64_t* head;       // [0] moves of a compaction, [1] free pages
+  int32_t* span_free;  // free pages of each span
+  int32_t* need;       // pages a request wants; -1: refused
+  int64_t* start;      // pages wanted by the requests before it
+  int32_t* free_list;  // free pages, ascending; a compaction's holes
+  int32_t* movers;     // a compaction's pages that move, descending, and their counts
+  int32_t* mover_refs;
+  int32_t* place;      // page -> its index among the movers, -1: none
+  int spans, span;
+};
+
+__device__ inline int clamped_length(const PageCache& c, int s) {
+  const int64_t most = (int64_t)c.max_pages * c.page_size;
+  const int64_t n = c.lengths[s];
+  return (int)(n < 0 ? 0 : n > most ? most : n);
+}
+__device__ inline int pages_of(const PageCache& c, int length) { return (int)(((int64_t)length + c.page_size - 1) / c.page_size); }
+__device__ inline bool is_page(const PageCache& c, int q) { return q >= 0 && q < c.num_pages; }
+__device__ inline void add_count(const PageCache& c, int q, int v) { atomicAdd(reinterpret_cast<uint32_t*>(c.refs) + q, (uint32_t)v); }
+
+// ---------------------------------------------------------------------------------------
+// Sums over the workgroup
+// ---------------------------------------------------------------------------------------
+struct BlockSum {
+  int64_t wave_total[kRequestWaves];
+};
+// exclusive prefix of v over the threads, and the total
+template <class T>
+__device__ inline T block_exclusive(BlockSum& sm, T v, T& total) {
+  const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const T incl = wave_inclusive_scan(v, T(0), [](T a, T b) { return a + b; });
+  __syncthreads();  // the last call's totals have been read
+  if (lane == kWave - 1) sm.wave_total[w] = incl;
+  __syncthreads();
+  T before = 0;
+  total = 0;
+#pragma unroll
+  for (int k = 0; k < kRequestWaves; k++) {
+    if (k < w) before += (T)sm.wave_total[k];
+    total += (T)sm.wave_total[k];
+  }
+  return before + incl - v;
+}
+// the sum of the positive ones of n values, the same in all threads
+__device__ inline int64_t block_sum(BlockSum& sm, const int32_t* v, int64_t n) {
+  int64_t mine = 0, total;
+  for (int64_t i = threadIdx.x; i < n; i += kPageBlock) mine += v[i] > 0 ? v[i] : 0;
+  block_exclusive(sm, mine, total);
+  return total;
+}
+
+// ---------------------------------------------------------------------------------------
+// Free pages
+// ---------------------------------------------------------------------------------------
+__device__ inline void tally_span(const PageCache& c, const PageTemp& t, int span) {
+  __shared__ BlockSum sm;
+  const int64_t begin = (int64_t)span * t.span;
+  const int64_t end = begin + t.span < c.num_pages ? begin + t.span : c.num_pages;
+  int mine = 0;
+  for (int64_t q = begin + threadIdx.x; q < end; q += kPageBlock) mine += c.refs[q] == 0;
+  int total;
+  block_exclusive(sm, mine, total);
+  if (threadIdx.x == 0) t.span_free[span] = total;
+}
+
+// f(q, count, free pages before q) for every page of a span, in all threads of the workgroup
+template <class F>
+__device__ inline void sweep_span(const PageCache& c, const PageTemp& t, BlockSum& sm, int span, int64_t before, F f) {
+  const int64_t begin = (int64_t)span * t.span;
+  const int64_t end = begin + t.span < c.num_pages ? begin + t.span : c.num_pages;
+  for (int64_t at = begin; at < end; at += kPageSweep) {
+    int n[kPagesPerThread];
+    const int64_t q0 = at + (int64_t)threadIdx.x * kPagesPerThread;
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPagesPerThread; k++) {
+      n[k] = q0 + k < end ? c.refs[q0 + k] : 1;
+      mine += n[k] == 0;
+    }
+    int total;
+    int64_t rank = before + block_exclusive(sm, mine, total);
+#pragma unroll
+    for (int k = 0; k < kPagesPerThread; k++) {
+      if (q0 + k < end) f(q0 + k, n[k], rank);
+      rank += n[k] == 0;
+    }
+    before += total;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Requests
+// ---------------------------------------------------------------------------------------
+// whether an earlier request names the same sequence (all lanes of a wavefront ask for the same one)
+__device__ inline bool named_before(const int32_t* named, int64_t i, int s) {
+  bool found = false;
+  for (int64_t q0 = 0; q0 < i; q0 += kWave) {
+    const int64_t q = q0 + lane_id();
+    found = found || (q < i && named[q] == s);
+  }
+  return __ballot(found) != 0;
+}
+__device__ inline bool named_anywhere(const int32_t* named, int64_t n, int s) { return named_before(named, n, s); }
+
+enum : int { kFork = 0, kForkShared = 1, kResize = 2 };
+
+struct Requests {
+  const int32_t* first;   // parents, or the lengths of a resize (NULL: 0)
+  const int32_t* named;   // children, or the sequences of a resize
+  int64_t n;
+  int kind;
+  uint8_t* done;
+};
+
+// Shrinks and frees.  need[i] = 0, or -1 where the request is refused.
+__global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, PageTemp t, Requests r) {
+  const int lane = lane_id();
+  const int64_t i = (int64_t)blockIdx.x * kRequestWaves + threadIdx.x / kWave;
+  if (i >= r.n) return;
+  const int s = r.named[i];
+  const int64_t want = r.first ? r.first[i] : 0;
+  bool ok = s >= 0 && s < c.num_sequences && want >= 0 && want <= (int64_t)c.max_pages * c.page_size;
+  if (ok) ok = !named_before(r.named, i, s);
+  if (lane == 0) {
+    if (t.need) t.need[i] = ok ? 0 : -1;
+    else if (r.done) r.done[i] = ok;  // pages_free: nothing is left to do
+  }
+  if (!ok) return;
+  const int old = __builtin_amdgcn_readfirstlane(clamped_length(c, s));
+  if (want >= old) return;
+  int32_t* row = c.tables + (int64_t)s * c.max_pages;
+  for (int j = pages_of(c, (int)want) + lane; j < pages_of(c, old); j += kWave) {
+    const int q = row[j];
+    if (is_page(c, q)) add_count(c, q, -1);
+    row[j] = -1;
+  }
+  if (lane == 0) c.lengths[s] = (int)want;
+}
+
+// the last page of a growing sequence when others name it too and something of it is free
+__device__ inline int page_to_copy(const PageCache& c, int s, int old, int want) {
+  if (want <= old || old % c.page_size == 0) return -1;
+  const int q = c.tables[(int64_t)s * c.max_pages + old / c.page_size];
+  return is_page(c, q) && c.refs[q] > 1 ? q : -1;
+}
+
+// Tallies the free pages and what each request wants.
+__global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, PageTemp t, Requests r) {
+  if ((int)blockIdx.x < t.spans) return tally_span(c, t, (int)blockIdx.x);
+  if (r.kind == kResize) {
+    const int64_t i = (int64_t)(blockIdx.x - t.spans) * kPageBlock + threadIdx.x;
+    if (i >= r.n || t.need[i] < 0) return;
+    const int s = r.named[i], old = clamped_length(c, s), want = r.first[i];
+    t.need[i] = want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (page_to_copy(c, s, old, want) >= 0);
+    return;
+  }
+  const int64_t i = (int64_t)(blockIdx.x - t.spans) * kRequestWaves + threadIdx.x / kWave;
+  if (i >= r.n) return;
+  const int parent = r.first[i], child = r.named[i];
+  bool ok = parent >= 0 && parent < c.num_sequences && child >= 0 && child < c.num_sequences;
+  if (ok) ok = c.lengths[child] == 0 && !named_before(r.named, i, child) && !named_anywhere(r.first, r.n, child);
+  int need = -1;
+  if (ok) {
+    const int n = clamped_length(c, parent);
+    need = r.kind == kForkShared ? (n % c.page_size != 0) : pages_of(c, n);
+  }
+  if (lane_id() == 0) t.need[i] = need;
+}
+
+// Lists the free pages, as many as are wanted, and adds up the requests.
+__global__ __launch_bounds__(kPageBlock) void pages_list_kernel(PageCache c, PageTemp t, int64_t n) {
+  __shared__ BlockSum sm;
+  if ((int)blockIdx.x == t.spans) {
+    int64_t sum = 0;
+    for (int64_t at = 0; at < n; at += kPageBlock) {
+      const int64_t i = at + threadIdx.x;
+      const int64_t need = i < n && t.need[i] > 0 ? t.need[i] : 0;
+      int64_t total;
+      const int64_t before = block_exclusive(sm, need, total);
+      if (i < n) t.start[i] = sum + before;
+      sum += total;
+    }
+    const int64_t free = block_sum(sm, t.span_free, t.spans);
+    if (threadIdx.x == 0) t.head[1] = free;
+    return;
+  }
+  const int64_t before = block_sum(sm, t.span_free, blockIdx.x);
+  const int64_t wanted = block_sum(sm, t.need, n);
+  if (before >= wanted) return;
+  sweep_span(c, t, sm, (int)blockIdx.x, before, [&](int64_t q, int count, int64_t rank) {
+    if (count == 0 && rank < wanted) t.free_list[rank] = (int)q;
+  });
+}
+
+// bytes [at, at + n) of a page, n <= kCopyUnit, by the whole workgroup
+__device__ inline void copy_unit(const char* from, char* to, int64_t at, int64_t n) {
+  const int nvec = (int)(n / 16);
+  tcd_v4u v[4];
+  if (n == kCopyUnit) {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      v[k] = __builtin_nontemporal_load(reinterpret_cast<const tcd_v4u_anywhere*>(from + at + (threadIdx.x + k * kPageBlock) * 16));
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      __builtin_nontemporal_store(v[k], reinterpret_cast<tcd_v4u_anywhere*>(to + at + (threadIdx.x + k * kPageBlock) * 16));
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int64_t i = threadIdx.x + k * kPageBlock;
+    if (i < nvec) v[k] = __builtin_nontemporal_load(reinterpret_cast<const tcd_v4u_anywhere*>(from + at + i * 16));
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int64_t i = threadIdx.x + k * kPageBlock;
+    if (i < nvec) __builtin_nontemporal_store(v[k], reinterpret_cast<tcd_v4u_anywhere*>(to + at + i * 16));
+  }
+  for (int64_t i = (int64_t)nvec * 16 + threadIdx.x; i < n; i += kPageBlock) to[at + i] = from[at + i];
+}
+__device__ inline void copy_page_unit(const PageCache& c, int pool, int from, int to, int64_t unit) {
+  const int64_t at = unit * kCopyUnit;
+  const int64_t n = c.page_bytes - at < kCopyUnit ? c.page_bytes - at : kCopyUnit;
+  char* base = reinterpret_cast<char*>(c.pools[pool]);
+  copy_unit(base + (int64_t)from * c.page_bytes, base + (int64_t)to * c.page_bytes, at, n);
+}
+
+// Serves the requests: workgroup (request, piece); piece 0 writes tables, counts and lengths, all of them copy.
+__global__ __launch_bounds__(kPageBlock) void pages_serve_kernel(PageCache c, PageTemp t, Requests r, int pieces) {
+  const int64_t i = blockIdx.x / (unsigned)pieces;
+  const int piece = (int)(blockIdx.x % (unsigned)pieces);
+  const int need = t.need[i];
+  const int64_t start = t.start[i];
+  const bool ok = need == 0 || (need > 0 && start + need <= t.head[1]);
+  if (piece == 0 && threadIdx.x == 0 && r.done) r.done[i] = ok;
+  if (!ok) return;
+  const int32_t* mine = t.free_list + start;
+  const int s = r.named[i];
+  int32_t* row = c.tables + (int64_t)s * c.max_pages;
+  const int64_t units = (c.page_bytes + kCopyUnit - 1) / kCopyUnit;
+
+  if (r.kind == kResize) {
+    const int want = r.first[i], old = clamped_length(c, s);
+    if (want <= old) return;
+    const int had = pages_of(c, old), have = pages_of(c, want), last = old / c.page_size;
+    const int own = need - (have - had);  // 1: a copy of the last page was asked for
+    const int q = own ? row[last] : -1;
+    __syncthreads();  // all threads have the old length and entry
+    if (own) {
+      for (int64_t u = 0; u < units * c.num_pools; u++) copy_page_unit(c, (int)(u / units), q, mine[0], u % units);
+    }
+    for (int j = had + (int)threadIdx.x; j < have; j += kPageBlock) {
+      const int page = mine[own + j - had];
+      row[j] = page;
+      c.refs[page] = 1;
+    }
+    if (threadIdx.x == 0) {
+      if (own) {
+        row[last] = mine[0];
+        c.refs[mine[0]] = 1;
+        add_count(c, q, -1);
+      }
+      c.lengths[s] = want;
+    }
+    return;
+  }
+  const int parent = r.first[i];
+  const int n = clamped_length(c, parent), held = pages_of(c, n);
+  const int32_t* from = c.tables + (int64_t)parent * c.max_pages;
+  const int shared = held - need;  // copies are the last pages
+  if (piece == 0) {
+    for (int j = threadIdx.x; j < held; j += kPageBlock) {
+      const int q = j < shared ? from[j] : mine[j - shared];
+      row[j] = q;
+      if (j >= shared) c.refs[q] = 1;
+      else if (is_page(c, q)) add_count(c, q, 1);
+    }
+    if (threadIdx.x == 0) c.lengths[s] = n;
+  }
+  const int64_t all = (int64_t)need * c.num_pools * units;
+  for (int64_t u = piece; u < all; u += pieces) {
+    const int64_t page = u / units;
+    const int j = (int)(page / c.num_pools);
+    const int q = from[shared + j];
+    if (is_page(c, q)) copy_page_unit(c, (int)(page % c.num_pools), q, mine[j], u % units);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Compaction.  With `live` pages in use, the free ones below `live` (holes) are as many as the ones in
+// use from there on (movers).  Holes are numbered from below by the free pages before them, movers
+// from above by the pages in use behind them; mover k moves to hole k.  No page is both.
+// ---------------------------------------------------------------------------------------
+__global__ __launch_bounds__(kPageBlock) void pages_tally_only_kernel(PageCache c, PageTemp t) { tally_span(c, t, (int)blockIdx.x); }
+
+__global__ __launch_bounds__(kPageBlock) void pages_rank_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
+  __shared__ BlockSum sm;
+  const int64_t before = block_sum(sm, t.span_free, blockIdx.x);
+  const int64_t live = c.num_pages - block_sum(sm, t.span_free, t.spans);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *live_out = (int)live;
+    if (live == c.num_pages) t.head[0] = 0;
+  }
+  sweep_span(c, t, sm, (int)blockIdx.x, before, [&](int64_t q, int count, int64_t rank) {
+    if (q == live) t.head[0] = rank;  // holes below
+    if (q < live) {
+      if (count == 0) t.free_list[rank] = (int)q;
+      else refs_out[q] = count;
+    } else {
+      int k = -1;
+      if (count != 0) {
+        k = (int)(live - 1 - (q - rank));
+        t.movers[k] = (int)q;
+        t.mover_refs[k] = count;
+      }
+      t.place[q] = k;
+      refs_out[q] = 0;
+    }
+  });
+}
+
+__global__ __launch_bounds__(kPageBlock) void pages_move_kernel(PageCache c, PageTemp t, int32_t* tables_out, int32_t* refs_out,
+                                                                const int32_t* live_at, int table_blocks) {
+  const int live = *live_at;
+  if ((int)blockIdx.x < table_blocks) {  // renumbers the tables
+    const int64_t all = (int64_t)c.num_sequences * c.max_pages;
+    for (int64_t e = (int64_t)blockIdx.x * kPageBlock + threadIdx.x; e < all; e += (int64_t)table_blocks * kPageBlock) {
+      int q = c.tables[e];
+      if (!is_page(c, q)) q = -1;
+      else if (q >= live) {
+        const int k = t.place[q];
+        q = k >= 0 ? t.free_list[k] : -1;
+      }
+      tables_out[e] = q;
+    }
+    return;
+  }
+  const int64_t moves = t.head[0];
+  const int64_t blocks = gridDim.x - table_blocks, block = blockIdx.x - table_blocks;
+  for (int64_t k = block * kPageBlock + threadIdx.x; k < moves; k += blocks * kPageBlock) refs_out[t.free_list[k]] = t.mover_refs[k];
+  const int64_t units = (c.page_bytes + kCopyUnit - 1) / kCopyUnit, all = moves * c.num_pools * units;
+  for (int64_t u = block; u < all; u += blocks) {
+    const int64_t page = u / units;
+    const int k = (int)(page / c.num_pools);
+    copy_page_unit(c, (int)(page % c.num_pools), t.movers[k], t.free_list[k], u % units);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------
+static bool cache_of(const thrust_cdna4_page_cache* a, PageCache& c) {
+  if (!a || a->num_pools < 0 || a->num_pages < 0 || a->page_bytes < 0 || a->page_size <= 0 || a->num_sequences < 0 || a->max_pages < 0) return false;
+  if ((int64_t)a->max_pages * a->page_size > 0x7fffffff) return false;  // lengths are 32-bit
+  c = PageCache{a->pools, a->page_bytes, a->num_pools, a->num_pages, a->page_size, a->num_sequences, a->max_pages, a->tables, a->lengths, a->refs};
+  return true;
+}
+static bool cache_usable(const PageCache& c) {
+  return (c.num_pages == 0 || c.refs) && (c.num_sequences == 0 || (c.lengths && (c.max_pages == 0 || c.tables))) &&
+         (c.num_pools == 0 || c.page_bytes == 0 || c.pools);
+}
+
+// carves the storage; returns its size
+static size_t page_temp(const PageCache& c, int64_t n, bool compact, void* temp, PageTemp& t) {
+  t.span = (int)(ceil_div(ceil_div(c.num_pages, (int64_t)kMaxSpans), (int64_t)kPageSweep) * kPageSweep);
+  if (t.span == 0) t.span = kPageSweep;
+  t.spans = (int)ceil_div(c.num_pages, (int64_t)t.span);
+  char* base = static_cast<char*>(temp);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* p = base ? base + at : nullptr;
+    at += align_up(bytes, 256);
+    return p;
+  };
+  t.head = reinterpret_cast<int64_t*>(take(16));
+  t.span_free = reinterpret_cast<int32_t*>(take((size_t)t.spans * 4));
+  t.need = reinterpret_cast<int32_t*>(take((size_t)n * 4));
+  t.start = reinterpret_cast<int64_t*>(take((size_t)n * 8));
+  t.free_list = reinterpret_cast<int32_t*>(take((size_t)c.num_pages * 4));
+  t.movers = t.mover_refs = t.place = nullptr;
+  if (compact) {
+    t.movers = reinterpret_cast<int32_t*>(take((size_t)c.num_pages * 4));
+    t.mover_refs = reinterpret_cast<int32_t*>(take((size_t)c.num_pages * 4));
+    t.place = reinterpret_cast<int32_t*>(take((size_t)c.num_pages * 4));
+  }
+  return at;
+}
+
+static hipError_t serve(const PageCache& c, const PageTemp& t, const Requests& r, hipStream_t s) {
+  const int64_t request_blocks = r.kind == kResize ? ceil_div(r.n, (int64_t)kPageBlock) : ceil_div(r.n, (int64_t)kRequestWaves);
+  TCD_LAUNCH("pages_tally_kernel", pages_tally_kernel, dim3((unsigned)(t.spans + request_blocks)), dim3(kPageBlock), s, c, t, r);
+  TCD_LAUNCH("pages_list_kernel", pages_list_kernel, dim3((unsigned)t.spans + 1u), dim3(kPageBlock), s, c, t, r.n);
+  int64_t pieces = 1;
+  if (r.kind != kResize) {  // enough workgroups to fill the device, none without a unit to copy
+    const int64_t units = ceil_div(c.page_bytes, (int64_t)kCopyUnit) * c.num_pools * (r.kind == kForkShared ? 1 : c.max_pages);
+    pieces = ceil_div((int64_t)device_cu_count() * 16, r.n);
+    if (pieces > units) pieces = units;
+    if (pieces < 1) pieces = 1;
+  }
+  TCD_LAUNCH("pages_serve_kernel", pages_serve_kernel, dim3((unsigned)(r.n * pieces)), dim3(kPageBlock), s, c, t, r, (int)pieces);
+  return hipGetLastError();
+}
+
+}  // namespace tcd
+
+extern "C" int thrust_cdna4_pages_fork(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, const int32_t* parents,
+                                       const int32_t* children, int64_t n, int share, uint8_t* done, void* stream) {
+  using namespace tcd;
+  PageCache c;
+  if (!temp_bytes || temp_misaligned(temp) || n < 0 || n > (1 << 24) || !cache_of(cache, c)) return hipErrorInvalidValue;
+  PageTemp t;
+  const size_t bytes = page_temp(c, n, false, temp, t);
+  if (!temp) {
+    *temp_bytes = bytes;
+    return hipSuccess;
+  }
+  if (n == 0) return hipSuccess;
+  if (*temp_bytes < bytes || !parents || !children || !done || !cache_usable(c)) return hipErrorInvalidValue;
+  return (int)serve(c, t, Requests{parents, children, n, share ? kForkShared : kFork, done}, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int thrust_cdna4_pages_resize(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, const int32_t* sequences,
+                                         const int32_t* lengths, int64_t n, uint8_t* done, void* stream) {
+  using namespace tcd;
+  PageCache c;
+  if (!temp_bytes || temp_misaligned(temp) || n < 0 || n > (1 << 24) || !cache_of(cache, c)) return hipErrorInvalidValue;
+  PageTemp t;
+  const size_t bytes = page_temp(c, n, false, temp, t);
+  if (!temp) {
+    *temp_bytes = bytes;
+    return hipSuccess;
+  }
+  if (n == 0) return hipSuccess;
+  if (*temp_bytes < bytes || !sequences || !lengths || !done || !cache_usable(c)) return hipErrorInvalidValue;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const Requests r{lengths, sequences, n, kResize, done};
+  TCD_LAUNCH("pages_shrink_kernel", pages_shrink_kernel, dim3((unsigned)ceil_div(n, (int64_t)kRequestWaves)), dim3(kPageBlock), s, c, t, r);
+  return (int)serve(c, t, r, s);
+}
+
+extern "C" int thrust_cdna4_pages_free(const thrust_cdna4_page_cache* cache, const int32_t* sequences, int64_t n, uint8_t* done, void* stream) {
+  using namespace tcd;
+  PageCache c;
+  if (n < 0 || n > (1 << 24) || !cache_of(cache, c)) return hipErrorInvalidValue;
+  if (n == 0) return hipSuccess;
+  if (!sequences || !cache_usable(c)) return hipErrorInvalidValue;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  TCD_LAUNCH("pages_shrink_kernel", pages_shrink_kernel, dim3((unsigned)ceil_div(n, (int64_t)kRequestWaves)), dim3(kPageBlock), s, c, PageTemp{},
+             (Requests{nullptr, sequences, n, kResize, done}));
+  return (int)hipGetLastError();
+}
+
+extern "C" int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, int32_t* tables_out,
+                                          int32_t* refs_out, int32_t* live_out, void* stream) {
+  using namespace tcd;
+  PageCache c;
+  if (!temp_bytes || temp_misaligned(temp) || !cache_of(cache, c)) return hipErrorInvalidValue;
+  PageTemp t;
+  const size_t bytes = page_temp(c, 0, true, temp, t);
+  if (!temp) {
+    *temp_bytes = bytes;
+    return hipSuccess;
+  }
+  const int64_t entries = (int64_t)c.num_sequences * c.max_pages;
+  if (*temp_bytes < bytes || !live_out || !cache_usable(c) || (c.num_pages > 0 && !refs_out) || (entries > 0 && !tables_out))
+    return hipErrorInvalidValue;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (c.num_pages == 0) {  // nothing to move; tables name nothing
+    hipError_t e = zero_async(live_out, 4, s);
+    if (e != hipSuccess) return (int)e;
+    e = zero_async(t.head, 16, s);
+    if (e != hipSuccess) return (int)e;
+  } else {
+    TCD_LAUNCH("pages_tally_only_kernel", pages_tally_only_kernel, dim3((unsigned)t.spans), dim3(kPageBlock), s, c, t);
+    TCD_LAUNCH("pages_rank_kernel", pages_rank_kernel, dim3((unsigned)t.spans), dim3(kPageBlock), s, c, t, refs_out, live_out);
+  }
+  int64_t table_blocks = ceil_div(entries, (int64_t)kPageBlock * 4);
+  if (table_blocks > 2048) table_blocks = 2048;
+  const int64_t units = ceil_div(c.page_bytes, (int64_t)kCopyUnit) * c.num_pools * (c.num_pages / 2);  // at most: half of the pages move
+  int64_t copy_blocks = (int64_t)device_cu_count() * 16;
+  if (copy_blocks > units) copy_blocks = units;
+  if (copy_blocks < 1) copy_blocks = 1;
+  TCD_LAUNCH("pages_move_kernel", pages_move_kernel, dim3((unsigned)(table_blocks + copy_blocks)), dim3(kPageBlock), s, c, t, tables_out,
+             refs_out, live_out, (int)table_blocks);
+  return (int)hipGetLastError();
+}

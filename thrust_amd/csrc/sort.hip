@@ -1119,9 +1119,10 @@ extern "C" int thrust_cdna4_lookback_timeout_counter(void** device_address) {
 
 extern "C" int thrust_cdna4_lookback_timeouts(unsigned long long* count) {
   if (!count) return hipErrorInvalidValue;
-  unsigned int c = 0;
-  const hipError_t e = hipMemcpyFromSymbol(&c, HIP_SYMBOL(tcd::g_lookback_timeouts), sizeof(c));
-  *count = c;
+  unsigned int c = 0, linear = 0;
+  hipError_t e = hipMemcpyFromSymbol(&c, HIP_SYMBOL(tcd::g_lookback_timeouts), sizeof(c));
+  if (e == hipSuccess) e = tcd::linear_scan_timeouts(&linear);
+  *count = (unsigned long long)c + linear;
   return (int)e;
 }
 

@@ -1,0 +1,127 @@
+"""Pages of a cache: sequences that share pages, grow, fork, end, and are closed up again.
+
+All of it is in device memory and nothing is read back: calls can be captured into a graph, and their
+effect depends on the contents of the arrays alone.  A page that no sequence names (refs 0) is free;
+requests take the lowest free pages in their order.
+"""
+import ctypes
+
+import torch
+
+from . import capi, device as dev
+
+
+class PageCache:
+    """`pools`: the arrays that are paged together (a layer's keys, its values, its recurrent states ...),
+    each [pages, ...], contiguous, of any type, with the same number of pages and of bytes a page.  A page
+    holds `page_size` tokens; for a state, which is never full, any number above the longest sequence.
+
+    tables  int32 [max_sequences, max_pages]  the pages of each sequence, -1 behind them
+    lengths int32 [max_sequences]             tokens; the first ceil(length / page_size) entries are held
+    refs    int32 [pages]                     how many tables name a page
+
+    They start empty, or are the given ones, which are then used in place.
+    """
+
+    def __init__(self, pools, page_size, max_sequences, max_pages, tables=None, lengths=None, refs=None):
+        pools = list(pools)
+        if not pools:
+            raise ValueError("a cache needs a pool")
+        device = dev.need_device(*pools, tables, lengths, refs)
+        for p in pools:
+            if p.dim() < 1 or not p.is_contiguous() or p.shape[0] != pools[0].shape[0]:
+                raise ValueError("pools must be contiguous and of the same number of pages")
+        page_bytes = {p[0].numel() * p.element_size() for p in pools} if pools[0].shape[0] else {0}
+        if len(page_bytes) > 1:
+            raise ValueError("pools must have the same number of bytes a page")
+        if page_size < 1 or max_sequences < 0 or max_pages < 0 or page_size * max_pages > 0x7fffffff:
+            raise ValueError("page_size must be positive, and page_size * max_pages below 2^31")
+        pages = pools[0].shape[0]
+        self.pools, self.page_size, self.device = pools, page_size, device
+        self.tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
+        self.lengths = self._array(lengths, (max_sequences,), 0, "lengths")
+        self.refs = self._array(refs, (pages,), 0, "refs")
+        self._pointers = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device)
+        self._args = capi.PageCacheArgs(pools=self._pointers.data_ptr(), page_bytes=page_bytes.pop(), num_pools=len(pools), num_pages=pages,
+                                        page_size=page_size, num_sequences=max_sequences, max_pages=max_pages,
+                                        tables=self.tables.data_ptr(), lengths=self.lengths.data_ptr(), refs=self.refs.data_ptr())
+        self._ref = ctypes.byref(self._args)
+        self._sizes = {}
+
+    def _array(self, given, shape, value, what):
+        if given is None:
+            return dev.empty(shape, torch.int32, self.device).fill_(value)
+        if given.dtype != torch.int32 or given.shape != shape or not given.is_contiguous():
+            raise ValueError(f"{what} must be int32 {list(shape)}, contiguous")
+        return given
+
+    def _requests(self, *ids):
+        if dev.need_device(*ids) != self.device:
+            raise ValueError("tensors on another device than the cache")
+        for t in ids:
+            if t.dtype != torch.int32 or t.dim() != 1 or t.shape != ids[0].shape or not t.is_contiguous():
+                raise ValueError("requests must be int32 vectors of one length, contiguous")
+        return ids[0].shape[0]
+
+    def _temp(self, entry, key, *args):
+        """Temporary storage for a call: asked for once, allocated each time (a graph keeps its own)."""
+        nbytes = self._sizes.get(key)
+        if nbytes is None:
+            nbytes = ctypes.c_size_t(0)
+            capi.check(entry(None, ctypes.byref(nbytes), self._ref, *args, None), key[0] + "(size)")
+            if len(self._sizes) > 256:
+                self._sizes.clear()
+            self._sizes[key] = nbytes
+        return dev.empty((nbytes.value,), torch.uint8, self.device), ctypes.byref(nbytes)
+
+    def resize(self, sequences, lengths):
+        """sequences[i] gets the length lengths[i] (int32 tensors).  Pages given up are there for the
+        sequences that grow; one that grows into a page which others name too gets its own copy of it.
+        Returns bool [n]: False where a request was refused (an id out of range, a sequence named
+        before, a length out of range, not enough free pages), which changes nothing of the sequence."""
+        n = self._requests(sequences, lengths)
+        L = capi.lib()
+        done = dev.empty((n,), torch.bool, self.device)
+        with dev.current(self.device):
+            temp, nbytes = self._temp(L.thrust_cdna4_pages_resize, ("pages_resize", n), None, None, n, None)
+            capi.check(L.thrust_cdna4_pages_resize(temp.data_ptr(), nbytes, self._ref, sequences.data_ptr(), lengths.data_ptr(), n,
+                                                   done.data_ptr(), dev.stream(self.device)), "pages_resize")
+        return done
+
+    def free(self, sequences):
+        """The sequences give back all their pages and are empty.  Ids out of range are passed over."""
+        n = self._requests(sequences)
+        with dev.current(self.device):
+            capi.check(capi.lib().thrust_cdna4_pages_free(self._ref, sequences.data_ptr(), n, None, dev.stream(self.device)), "pages_free")
+
+    def fork(self, parents, children, share=True):
+        """Sequence children[i], which must be empty and no parent in the call, becomes a copy of
+        parents[i]: with `share` it names the parent's full pages and gets a copy of the partly filled
+        one, otherwise copies of all.  Returns bool [n]: False where refused (an id out of range, a child
+        that is not empty, a parent or named before, not enough free pages)."""
+        n = self._requests(parents, children)
+        L = capi.lib()
+        done = dev.empty((n,), torch.bool, self.device)
+        with dev.current(self.device):
+            temp, nbytes = self._temp(L.thrust_cdna4_pages_fork, ("pages_fork", n), None, None, n, 0, None)
+            capi.check(L.thrust_cdna4_pages_fork(temp.data_ptr(), nbytes, self._ref, parents.data_ptr(), children.data_ptr(), n, bool(share),
+                                                 done.data_ptr(), dev.stream(self.device)), "pages_fork")
+        return done
+
+    def compact(self, tables=None, refs=None):
+        """Moves pages until those in use are the lowest, and renumbers.  Returns their number, int32 [1].
+        With `tables` and `refs` the new ones go there and the cache's own stay as they are: the pages
+        moved from keep their contents, so work in flight with the old tables may end."""
+        if (tables is None) != (refs is None):
+            raise ValueError("tables and refs go together")
+        if dev.need_device(tables, refs) not in (None, self.device):
+            raise ValueError("tensors on another device than the cache")
+        tables = self.tables if tables is None else self._array(tables, self.tables.shape, None, "tables")
+        refs = self.refs if refs is None else self._array(refs, self.refs.shape, None, "refs")
+        L = capi.lib()
+        live = dev.empty((1,), torch.int32, self.device)
+        with dev.current(self.device):
+            temp, nbytes = self._temp(L.thrust_cdna4_pages_compact, ("pages_compact",), None, None, None)
+            capi.check(L.thrust_cdna4_pages_compact(temp.data_ptr(), nbytes, self._ref, tables.data_ptr(), refs.data_ptr(), live.data_ptr(),
+                                                    dev.stream(self.device)), "pages_compact")
+        return live

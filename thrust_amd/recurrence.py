@@ -1,0 +1,164 @@
+"""Gated linear recurrence: h[t] = a[t] * h[t-1] + x[t] for every channel, its gradient, and its step
+for single tokens.  A scan, as thrust::inclusive_scan is, of affine maps along the rows.
+
+Gates and inputs are [batch, rows, channels], or packed [rows, channels] with `offsets` [sequences + 1]
+(int32 or int64, ascending; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none).
+Channels are next to each other; batches and rows may have any strides, as the halves of one projection
+have.  x is float32, float16 or bfloat16, gates are of the same type or float32; with log_gate they are
+logarithms of the factors.  States are float32 [sequences or batch, channels].  Sums are in 32 bits and
+rounded once.
+"""
+import ctypes
+
+import torch
+
+from . import capi, device as dev
+
+_DT = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+
+
+def _types(gate, x):
+    if x.dtype not in _DT or gate.dtype not in (x.dtype, torch.float32):
+        raise ValueError("x must be float32, float16 or bfloat16, and the gates of its type or float32")
+
+
+def _rows(t, shape, what):
+    """(batch stride, row stride) of a tensor of this shape."""
+    if t.shape != shape:
+        raise ValueError(f"{what} must have the shape of x")
+    if t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
+        raise ValueError(f"{what}: channels must be next to each other")
+    return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+
+
+def _distinct(t, what):
+    """Refuses an output whose elements share memory."""
+    need = t.shape[-1]
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1), key=lambda v: v[1]):
+        if stride < need:
+            raise ValueError(f"{what}: rows overlap")
+        need = stride * (size - 1) + need
+
+
+def _state(t, sequences, channels, what):
+    if t is None:
+        return
+    if t.dtype != torch.float32 or t.shape != (sequences, channels) or not t.is_contiguous():
+        raise ValueError(f"{what} must be float32 [{sequences}, {channels}], contiguous")
+
+
+def _shape(gate, x, offsets, log_gate):
+    """The arguments that say what is computed, the number of sequences and of chunks."""
+    _types(gate, x)
+    if offsets is None:
+        if x.dim() != 3:
+            raise ValueError("x must be [batch, rows, channels], or [rows, channels] with offsets")
+        batch, rows, channels = x.shape
+        sequences, size = batch, 0
+    else:
+        if x.dim() != 2:
+            raise ValueError("x must be [rows, channels] where offsets are given")
+        if offsets.dim() != 1 or offsets.dtype not in (torch.int32, torch.int64) or not offsets.is_contiguous() or offsets.numel() < 1:
+            raise ValueError("offsets must be int32 or int64 [sequences + 1], contiguous")
+        batch, (rows, channels) = 1, x.shape
+        sequences, size = offsets.numel() - 1, offsets.element_size()
+    fields = dict(gate_dtype=_DT[gate.dtype], x_dtype=_DT[x.dtype], log_gate=bool(log_gate), offset_bytes=size,
+                  batch=batch, rows=rows, channels=channels, sequences=sequences, offsets=dev.pointer(offsets))
+    return fields, sequences, (batch, -(-rows // capi.LINEAR_SCAN_CHUNK), channels)
+
+
+def _strided(fields, name, t, shape):
+    fields[name] = t.data_ptr()
+    fields[name + "_batch_stride"], fields[name + "_row_stride"] = _rows(t, shape, name)
+
+
+def _run(entry, args, device, what):
+    with dev.current(device):
+        nbytes = ctypes.c_size_t(0)
+        stream = dev.stream(device)
+        capi.check(entry(None, ctypes.byref(nbytes), ctypes.byref(args), stream), what + "(size)")
+        temp = dev.empty((nbytes.value,), torch.uint8, device)
+        capi.check(entry(temp.data_ptr(), ctypes.byref(nbytes), ctypes.byref(args), stream), what)
+
+
+def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, return_states=False):
+    """h[t] = a[t] * h[t-1] + x[t]; returns (out, final): every h in the type of x, and the last one of
+    each sequence in float32.  `init`: the states before the first rows (zero if None).  `out` may be x
+    or gate.  return_states: also the state that enters each chunk of 64 rows, for linear_scan_backward.
+    Packed rows that belong to no sequence are left as they were in a given `out`, and zero in a new one."""
+    device = dev.need_device(gate, x, init, offsets, out)
+    dev.no_autograd(gate, x, init)
+    fields, sequences, chunks = _shape(gate, x, offsets, log_gate)
+    _state(init, sequences, x.shape[-1], "init")
+    fields["clear_outside"] = out is None
+    if out is None:
+        out = dev.empty(x.shape, x.dtype, device)
+    else:
+        if out.dtype != x.dtype:
+            raise ValueError("out must have the type of x")
+        _distinct(out, "out")
+    _strided(fields, "gate", gate, x.shape)
+    _strided(fields, "x", x, x.shape)
+    _strided(fields, "out", out, x.shape)
+    final = dev.empty((sequences, x.shape[-1]), torch.float32, device)
+    states = dev.empty(chunks, torch.float32, device) if return_states else None
+    args = capi.LinearScanArgs(init=dev.pointer(init), final_state=final.data_ptr(), states=dev.pointer(states), **fields)
+    _run(capi.lib().thrust_cdna4_linear_scan, args, device, "linear_scan")
+    return (out, final, states) if return_states else (out, final)
+
+
+def linear_scan_backward(grad_out, gate, x, states, init=None, grad_final=None, offsets=None, log_gate=False):
+    """The gradient of linear_scan for the gradients of its out and final (zero if None): returns
+    (grad_gate, grad_x, grad_init), in the types of gate, x and init (None if there is no init).
+    `states` are those that linear_scan returned."""
+    device = dev.need_device(grad_out, gate, x, states, init, grad_final, offsets)
+    dev.no_autograd(grad_out, gate, x, init, grad_final)
+    fields, sequences, chunks = _shape(gate, x, offsets, log_gate)
+    _state(init, sequences, x.shape[-1], "init")
+    _state(grad_final, sequences, x.shape[-1], "grad_final")
+    if states.dtype != torch.float32 or states.shape != chunks or not states.is_contiguous():
+        raise ValueError("states must be what linear_scan returned for these shapes")
+    if grad_out.dtype != x.dtype:
+        raise ValueError("grad_out must have the type of x")
+    grad_gate, grad_x = dev.empty(x.shape, gate.dtype, device), dev.empty(x.shape, x.dtype, device)
+    grad_init = None if init is None else dev.empty(init.shape, torch.float32, device)
+    fields["clear_outside"] = True
+    for name, t in (("gate", gate), ("x", x), ("grad_out", grad_out), ("grad_gate", grad_gate), ("grad_x", grad_x)):
+        _strided(fields, name, t, x.shape)
+    args = capi.LinearScanBackwardArgs(init=dev.pointer(init), states=states.data_ptr(), grad_final=dev.pointer(grad_final),
+                                       grad_init=dev.pointer(grad_init), **fields)
+    _run(capi.lib().thrust_cdna4_linear_scan_backward, args, device, "linear_scan_backward")
+    return grad_gate, grad_x, grad_init
+
+
+def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
+    """One row for each of a batch: state[slots[i]] = a[i] * state[slots[i]] + x[i], in place; returns the
+    new states in the type of x.  gate and x are [batch, channels], state float32 [slots, channels],
+    slots int32 [batch] (None: row i has slot i).  A slot outside the cache marks a padded row, whose out
+    is zero.  Rows of one slot are taken in their order.  `out` may be x or gate."""
+    device = dev.need_device(gate, x, state, slots, out)
+    dev.no_autograd(gate, x, state)
+    _types(gate, x)
+    if x.dim() != 2:
+        raise ValueError("x must be [batch, channels]")
+    batch, channels = x.shape
+    if state.dim() != 2:
+        raise ValueError("state must be [slots, channels]")
+    _state(state, state.shape[0], channels, "state")
+    if slots is None:
+        if batch > state.shape[0]:
+            raise ValueError("more rows than slots")
+    elif slots.dtype != torch.int32 or slots.shape != (batch,) or not slots.is_contiguous():
+        raise ValueError("slots must be int32 [batch], contiguous")
+    if out is None:
+        out = dev.empty(x.shape, x.dtype, device)
+    else:
+        if out.dtype != x.dtype:
+            raise ValueError("out must have the type of x")
+        _distinct(out, "out")
+    with dev.current(device):
+        capi.check(capi.lib().thrust_cdna4_linear_scan_step(
+            _DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate.data_ptr(), _rows(gate, x.shape, "gate")[1], x.data_ptr(), _rows(x, x.shape, "x")[1],
+            out.data_ptr(), _rows(out, x.shape, "out")[1], state.data_ptr(), state.shape[0], dev.pointer(slots), batch, channels,
+            dev.stream(device)), "linear_scan_step")
+    return out
