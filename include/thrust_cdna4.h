@@ -188,7 +188,7 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  * columns.  a[t] is gate[t], or exp(gate[t]) when `log_gate` is not 0.
  *
  * Shapes: `batch` sequences of `rows` rows of `channels` elements; element (b, t, c) of an array is
- * at b * batch_stride + t * row_stride + c (strides in elements, not negative).  Or packed:
+ * at b * batch_stride + t * row_stride + c (strides in elements, not negative; at most 2^28 channels).  Or packed:
  * `offset_bytes` 4 or 8, `offsets` a DEVICE array of sequences + 1 ascending signed integers of that
  * size, batch 1; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none.  Rows
  * in front of the first sequence and behind the last one are part of none: their outputs are left as

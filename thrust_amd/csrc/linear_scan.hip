@@ -39,6 +39,7 @@ constexpr int kLinBlock = kLinWaves * kWave;
 constexpr int kLinGroup = 8;   // tiles of a group, groups of a super-group
 constexpr int kLinSuper = kLinGroup * kLinGroup;
 constexpr int kLinChunk = THRUST_CDNA4_LINEAR_SCAN_CHUNK;
+constexpr int64_t kLinMaxChannels = int64_t(1) << 28;  // a lane's offset in a row of maps is 32 bits of bytes
 constexpr uint32_t kLinSpinLimit = 1u << 22;
 
 __device__ unsigned int g_linear_scan_timeouts;
@@ -69,28 +70,10 @@ struct LinArgs {
 // ---------------------------------------------------------------------------------------
 __device__ inline uint32_t canonical_bits(float v) { return v != v ? 0x7fc00000u : bit_cast<uint32_t>(v); }
 
-__device__ inline void publish_map(uint64_t* p, float a, float h) {
-  st_agent(p, ~(((uint64_t)canonical_bits(a) << 32) | canonical_bits(h)));
-}
-
-// The ticket order makes every predecessor a running workgroup, so these waits end; the limit keeps a
-// mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts).
-template <int VEC, class W>
-__device__ inline void wait_words(const W* p, W (&v)[VEC]) {
-  for (uint32_t spins = 0;; spins++) {
-    bool all = true;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) v[j] = ld_agent(p + j);
-#pragma unroll
-    for (int j = 0; j < VEC; j++) all = all && v[j] != 0;
-    if (all) break;
-    if (spins >= kLinSpinLimit) {
-      atomicAdd(&g_linear_scan_timeouts, 1u);
-      break;
-    }
-    __builtin_amdgcn_s_sleep(1);
-  }
-}
+struct Map {
+  float a, h;
+};
+__device__ inline void publish_map(uint64_t* p, Map m) { st_agent(p, ~(((uint64_t)canonical_bits(m.a) << 32) | canonical_bits(m.h))); }
 
 // ---------------------------------------------------------------------------------------
 // Sequences of packed rows.  Everything here is the same in all lanes of a wavefront.  Offsets that
@@ -178,20 +161,34 @@ __device__ inline void previous_sequence(const LinArgs& p, int64_t row, int& s) 
   }
 }
 
+// A row's element c of this lane: the row's address is the same in all lanes and stays in scalar
+// registers, what differs is 32 bits of offset.
+template <class T>
+__device__ inline T* at(T* row, uint32_t c) {
+  using Byte = typename std::conditional<std::is_const<T>::value, const char, char>::type;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + c * (uint32_t)sizeof(T));
+}
+__device__ inline int64_t first_lane(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 template <int VEC>
-__device__ inline void load_state(const float* p, int64_t at, float (&h)[VEC]) {
+__device__ inline void load_state(const float* p, int64_t row, uint32_t c, float (&h)[VEC]) {
   if (p) {
+    p = at(p + row, c);
 #pragma unroll
-    for (int j = 0; j < VEC; j++) h[j] = p[at + j];
+    for (int j = 0; j < VEC; j++) h[j] = p[j];
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; j++) h[j] = 0.f;
   }
 }
 template <int VEC>
-__device__ inline void store_state(float* p, int64_t at, const float (&h)[VEC]) {
+__device__ inline void store_state(float* p, int64_t row, uint32_t c, const float (&h)[VEC]) {
+  p = at(p + row, c);
 #pragma unroll
-  for (int j = 0; j < VEC; j++) p[at + j] = h[j];
+  for (int j = 0; j < VEC; j++) p[j] = h[j];
 }
 
 // ---------------------------------------------------------------------------------------
@@ -200,10 +197,10 @@ __device__ inline void store_state(float* p, int64_t at, const float (&h)[VEC]) 
 // ---------------------------------------------------------------------------------------
 template <int CH>
 struct LinShared {
-  float a[kLinWaves][CH], h[kLinWaves][CH];    // maps of the tile's wavefronts
-  float pa[kLinWaves][CH], ph[kLinWaves][CH];  // maps of earlier tiles, then of earlier groups
-  float state[CH];                             // state of the super-group before
-  float carry[CH];
+  float a[kLinWaves][CH], h[kLinWaves][CH];  // maps of the tile's wavefronts
+  float map_a[CH], map_h[CH];                // the map of the group's earlier tiles
+  float carry[CH];                           // the state before them
+  int in_group;                              // the sequence begins among them: map_h is a state, and all there is
   int anew[kLinWaves];  // wavefront: a sequence begins in it (its h is then a state)
   int64_t since;        // logical row in which the sequence of the tile's first row begins; -1: none comes in
   uint32_t ticket;
@@ -217,116 +214,112 @@ __device__ inline void fold(const float (*a)[CH], const float (*h)[CH], int m0, 
     A *= a[m][ch];
   }
 }
+__device__ inline float map_factor(uint64_t word) { return bit_cast<float>((uint32_t)(~word >> 32)); }
+__device__ inline float map_shift(uint64_t word) { return bit_cast<float>((uint32_t)~word); }
+
+// Waits until n words that start `stride` elements apart are published; they have been asked for once.
+template <int N, class W>
+__device__ inline void wait_words(const W* p, int64_t stride, uint32_t c, W (&v)[N]) {
+  // The ticket order makes every predecessor a running workgroup, so these waits end; the limit keeps a
+  // mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts).
+  for (uint32_t spins = 0;; spins++) {
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < N; k++) all = all && v[k] != 0;
+    if (all) return;
+    if (spins >= kLinSpinLimit) break;
+    __builtin_amdgcn_s_sleep(1);
+#pragma unroll
+    for (int k = 0; k < N; k++)
+      if (v[k] == 0) v[k] = ld_agent(at(p + k * stride, c));
+  }
+  atomicAdd(&g_linear_scan_timeouts, 1u);
+}
 
 // Called by the whole workgroup after sm.a, sm.h, sm.anew and sm.since are written and a barrier.
-// `i`: logical tile of `nt`; `rows`: rows of a tile.  Leaves the entering state in sm.carry.
+// `i`: logical tile of `nt`; `rows`: rows of a tile.  Leaves the map of the group's earlier tiles in
+// sm.map_a and sm.map_h and the state before them in sm.carry.  One half of the workgroup deals with the
+// tiles of the group and the other with what lies before it, a thread for each channel; what a thread
+// may wait for it asks for at once, so that maps which are there cost one trip to memory.
 template <int VEC>
-__device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, int b, int64_t i, int64_t nt, int rows, int64_t c0, bool active,
-                                  int64_t block_c0) {
-  constexpr int CH = kWave * VEC;
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+__device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, int b, int64_t i, int64_t nt, int rows, int64_t block_c0) {
+  constexpr int CH = kWave * VEC, N = kLinGroup - 1;
+  const int ch = threadIdx.x % CH, role = __builtin_amdgcn_readfirstlane((int)threadIdx.x / CH);
   const int64_t C = p.channels, groups = ceil_div(nt, kLinGroup), supers = ceil_div(nt, kLinSuper);
   const bool publishes = i + 1 < nt;
-  const int64_t since = sm.since;
-  const bool needs = since >= 0;             // a sequence comes in from earlier tiles
+  const int64_t since = first_lane(sm.since);
+  const bool needs = since >= 0;                   // a sequence comes in from earlier tiles
   const int64_t first = needs ? since / rows : i;  // the tile it begins in
-  const int64_t g = i / kLinGroup, base = g * kLinGroup, sg = g / kLinGroup;
-
+  const int64_t g = i / kLinGroup, base = g * kLinGroup, sg = g / kLinGroup, gbase = sg * kLinGroup, gfirst = first / kLinGroup;
+  const bool in_group = needs && first >= base;
+  const int64_t from = block_c0 + ch / VEC * VEC;
+  const uint32_t chan = (uint32_t)((from + VEC > C ? C - VEC : from) + ch % VEC);
   int last_anew = -1;
 #pragma unroll
   for (int v = 0; v < kLinWaves; v++)
     if (sm.anew[v]) last_anew = v;
-  // the tile's own map for channel ch (a state, with A unused, where a sequence begins in it)
-  auto tile_total = [&](int ch, float& A, float& H) {
-    A = 1.f;
-    H = last_anew >= 0 ? sm.h[last_anew][ch] : 0.f;
+  last_anew = __builtin_amdgcn_readfirstlane(last_anew);
+  // the tile's own map after (A, H); folded again where it is needed again, which is rare, rather than
+  // kept in registers over the waits
+  auto tile_after = [&](float A, float H) {
+    if (last_anew >= 0) H = sm.h[last_anew][ch];
     fold<CH>(sm.a, sm.h, last_anew + 1, kLinWaves, ch, A, H);
+    return Map{A, H};
   };
-  // the last wavefront publishes the tile's map, the others wait for those of the group
-  if (w == kLinWaves - 1) {
-    if (publishes && active) {
+  if (role == 0 && from < C) {
+    if (publishes) publish_map(at(p.tile_map + ((int64_t)b * nt + i) * C, chan), tile_after(1.f, 0.f));
+    __builtin_amdgcn_sched_barrier(0);  // the folded maps' registers are free for the words that follow
+    const uint64_t* maps = p.tile_map + ((int64_t)b * nt + base) * C;
+    const int k0 = needs ? (int)(in_group ? first - base : 0) : N, k1 = (int)(i - base);
+    uint64_t v[N];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        float A, H;
-        tile_total(lane * VEC + j, A, H);
-        publish_map(p.tile_map + ((int64_t)b * nt + i) * C + c0 + j, A, H);
+    for (int k = 0; k < N; k++) v[k] = k >= k0 && k < k1 ? ld_agent(at(maps + k * C, chan)) : ~uint64_t(0);
+    wait_words(maps, C, chan, v);
+    // (GA, GH): the map of the group's earlier tiles, or GH a state where the sequence begins among them
+    float GA = 1.f, GH = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if (k >= k0 && k < k1) {
+        const float a = map_factor(v[k]), h = map_shift(v[k]);
+        GH = in_group && k == k0 ? h : a * GH + h;
+        GA = in_group && k == k0 ? 0.f : GA * a;
       }
     }
-  } else if (needs && base + w < i && base + w >= first && active) {
-    uint64_t v[VEC];
-    wait_words<VEC>(p.tile_map + ((int64_t)b * nt + base + w) * C + c0, v);
+    if (publishes && i - base == N)
+      publish_map(at(p.group_map + ((int64_t)b * groups + g) * C, chan), tile_after(GA, GH));
+    sm.map_a[ch] = GA;
+    sm.map_h[ch] = GH;
+  } else if (role == 1 && from < C) {
+    float H = 0.f;
+    if (needs && !in_group) {
+      const uint64_t* maps = p.group_map + ((int64_t)b * groups + gbase) * C;
+      const uint32_t* states = p.super_state + ((int64_t)b * supers + sg - 1) * C;
+      const bool from_super = gfirst < gbase;
+      const int k0 = from_super ? 0 : (int)(gfirst - gbase), k1 = (int)(g - gbase);
+      uint64_t v[N];
+      uint32_t state[1] = {~0u};
 #pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      sm.pa[w][lane * VEC + j] = bit_cast<float>((uint32_t)(~v[j] >> 32));
-      sm.ph[w][lane * VEC + j] = bit_cast<float>((uint32_t)~v[j]);
+      for (int k = 0; k < N; k++) v[k] = k >= k0 && k < k1 ? ld_agent(at(maps + k * C, chan)) : ~uint64_t(0);
+      if (from_super) state[0] = ld_agent(at(states, chan));
+      wait_words(maps, C, chan, v);
+      wait_words(states, 0, chan, state);
+      H = bit_cast<float>(~state[0]);
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        if (k >= k0 && k < k1) {
+          const float a = map_factor(v[k]), h = map_shift(v[k]);
+          H = !from_super && k == k0 ? h : a * H + h;
+        }
+      }
     }
+    sm.carry[ch] = H;
   }
+  if (threadIdx.x == 0) sm.in_group = in_group;
   __syncthreads();
-  // a thread for each channel from here on; (GA, GH) is the map of the group's earlier tiles, or GH a state
-  const int ch = tid;
-  const int64_t chan = [&] {
-    const int64_t at = block_c0 + ch / VEC * VEC;
-    return (at + VEC > C ? C - VEC : at) + ch % VEC;
-  }();
-  const bool mine = ch < CH && block_c0 + ch / VEC * VEC < C;
-  const bool in_group = needs && first >= base;
-  float GA = 1.f, GH = 0.f;
-  if (mine) {
-    if (in_group && i > base) {
-      GH = sm.ph[first - base][ch];
-      fold<CH>(sm.pa, sm.ph, (int)(first - base) + 1, (int)(i - base), ch, GA, GH);
-    } else if (needs) {
-      fold<CH>(sm.pa, sm.ph, 0, (int)(i - base), ch, GA, GH);
-    }
-    if (publishes && i - base == kLinGroup - 1) {
-      float A, H;
-      tile_total(ch, A, H);
-      if (last_anew < 0) {
-        H = A * GH + H;
-        A *= GA;
-      }
-      publish_map(p.group_map + ((int64_t)b * groups + g) * C + chan, A, H);
-    }
+  if (role == 0 && from < C && publishes && i % kLinSuper == kLinSuper - 1) {
+    const float H = in_group ? sm.map_h[ch] : sm.map_a[ch] * sm.carry[ch] + sm.map_h[ch];
+    st_agent(at(p.super_state + ((int64_t)b * supers + sg) * C, chan), ~canonical_bits(tile_after(1.f, H).h));
   }
-  if (needs && !in_group) {
-    __syncthreads();  // pa and ph are free again
-    const int64_t gbase = sg * kLinGroup, gfirst = first / kLinGroup;
-    if (w == kLinWaves - 1) {
-      if (gfirst < gbase && active) {
-        uint32_t v[VEC];
-        wait_words<VEC>(p.super_state + ((int64_t)b * supers + sg - 1) * C + c0, v);
-#pragma unroll
-        for (int j = 0; j < VEC; j++) sm.state[lane * VEC + j] = bit_cast<float>(~v[j]);
-      }
-    } else if (gbase + w < g && gbase + w >= gfirst && active) {
-      uint64_t v[VEC];
-      wait_words<VEC>(p.group_map + ((int64_t)b * groups + gbase + w) * C + c0, v);
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        sm.pa[w][lane * VEC + j] = bit_cast<float>((uint32_t)(~v[j] >> 32));
-        sm.ph[w][lane * VEC + j] = bit_cast<float>((uint32_t)~v[j]);
-      }
-    }
-    __syncthreads();
-    if (mine) {
-      float A = 1.f, H;
-      int from = 0;
-      if (gfirst < gbase) H = sm.state[ch];
-      else H = sm.ph[gfirst - gbase][ch], from = (int)(gfirst - gbase) + 1;
-      fold<CH>(sm.pa, sm.ph, from, (int)(g - gbase), ch, A, H);
-      GH = GA * H + GH;
-    }
-  }
-  if (mine) {
-    sm.carry[ch] = GH;
-    if (publishes && i % kLinSuper == kLinSuper - 1) {
-      float A, H;
-      tile_total(ch, A, H);
-      if (last_anew < 0) H = A * GH + H;
-      st_agent(p.super_state + ((int64_t)b * supers + sg) * C + chan, ~canonical_bits(H));
-    }
-  }
-  __syncthreads();
 }
 
 // The state that enters logical wavefront `lw` of the tile
@@ -335,11 +328,12 @@ __device__ inline void wave_carry(const LinShared<kWave * VEC>& sm, int lw, int 
   int last_anew = -1;
   for (int v = 0; v < lw; v++)
     if (sm.anew[v]) last_anew = v;
+  last_anew = __builtin_amdgcn_readfirstlane(last_anew);
 #pragma unroll
   for (int j = 0; j < VEC; j++) {
     const int ch = lane * VEC + j;
     float A = 1.f;
-    h[j] = last_anew >= 0 ? sm.h[last_anew][ch] : sm.carry[ch];
+    h[j] = last_anew >= 0 ? sm.h[last_anew][ch] : sm.in_group ? sm.map_h[ch] : sm.map_a[ch] * sm.carry[ch] + sm.map_h[ch];
     fold<kWave * VEC>(sm.a, sm.h, last_anew + 1, lw, ch, A, h[j]);
   }
 }
@@ -351,7 +345,7 @@ __device__ inline void take_lin_tile(const LinArgs& p, uint32_t* shared, int64_t
   if (p.ticket) {
     if (threadIdx.x == 0) *shared = atomicAdd(p.ticket, 1u);
     __syncthreads();
-    t = *shared;
+    t = (uint32_t)__builtin_amdgcn_readfirstlane((int)*shared);
   }
   const uint32_t across = (uint32_t)p.batch * (uint32_t)p.ncb;
   i = t / across;
@@ -362,17 +356,32 @@ __device__ inline void take_lin_tile(const LinArgs& p, uint32_t* shared, int64_t
 
 // States of sequences without rows: the final state is the initial one (the gradients likewise).
 template <int VEC>
-__device__ inline void empty_sequences(const LinArgs& p, int64_t i, const float* from, float* to, int64_t c0, bool active) {
+__device__ inline void empty_sequences(const LinArgs& p, int64_t i, const float* from, float* to, uint32_t c0, bool active) {
   const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   for (int64_t s0 = (i * kLinWaves + w) * kWave; s0 < p.sequences; s0 += (int64_t)p.ntiles * kLinWaves * kWave) {
     const int64_t s = s0 + lane;
     uint64_t none = __ballot(s < p.sequences && offset_at(p, s) >= offset_at(p, s + 1));
     while (none) {
-      const int64_t at = (s0 + __builtin_ctzll(none)) * p.channels + c0;
+      const int64_t row = (s0 + __builtin_ctzll(none)) * p.channels;
       none &= none - 1;
       float h[VEC];
-      load_state<VEC>(from, at, h);
-      if (active) store_state<VEC>(to, at, h);
+      load_state<VEC>(from, row, c0, h);
+      if (active) store_state<VEC>(to, row, c0, h);
+    }
+  }
+}
+
+// 32-bit gates that are logarithms are replaced once, where they are; 16-bit ones, whose factors do not
+// fit their place, are taken through exp in each pass of kernels of their own (LOG16; left to a test at
+// run time the exponentials were computed for every gate and cost as much as the memory traffic).
+template <class TG, int VEC, int S>
+__device__ inline void gates_of_logarithms(const LinArgs& p, Pack<TG, VEC> (&gate)[S]) {
+  if constexpr (sizeof(TG) == 4) {
+    if (p.log_gate) {
+#pragma unroll
+      for (int k = 0; k < S; k++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) gate[k].w[j] = bit_cast<uint32_t>(expf(gate[k].value(j)));
     }
   }
 }
@@ -380,7 +389,7 @@ __device__ inline void empty_sequences(const LinArgs& p, int64_t i, const float*
 // ---------------------------------------------------------------------------------------
 // The recurrence
 // ---------------------------------------------------------------------------------------
-template <class TG, class TX, int VEC, int S, bool PACKED>
+template <class TG, class TX, int VEC, int S, bool PACKED, bool LOG16>
 __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   constexpr int CH = kWave * VEC, R = S * kLinWaves;
   __shared__ LinShared<CH> sm;
@@ -391,30 +400,32 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   const int64_t C = p.channels, block_c0 = (int64_t)cb * CH;
   // the last lane's vector ends with the last channel: it may repeat channels of the lane before it,
   // and stores the same values
-  const int64_t at = block_c0 + lane * VEC;
-  const bool active = at < C;
-  const int64_t c0 = at + VEC > C ? C - VEC : at;
+  const int64_t from = block_c0 + lane * VEC;
+  const bool active = from < C;
+  const uint32_t c0 = (uint32_t)(from + VEC > C ? C - VEC : from);
   const int64_t r0 = i * R + w * S;
-  const int64_t left = p.rows - r0;
+  const int64_t rows_left = p.rows - r0;
+  const int left = rows_left < 0 ? 0 : rows_left < S ? (int)rows_left : S;  // of this wavefront's S
 
   Pack<TG, VEC> gate[S];
   Pack<TX, VEC> x[S];
   if (left > 0) {
-    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + c0;
-    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + c0;
+    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + r0 * p.gate_rs;
+    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + r0 * p.x_rs;
 #pragma unroll
     for (int k = 0; k < S; k++) {
-      const int64_t row = k < left ? r0 + k : p.rows - 1;
-      gate[k] = load_pack<TG, VEC>(gp + row * p.gate_rs);
-      x[k] = load_pack<TX, VEC>(xp + row * p.x_rs);
+      gate[k] = load_pack<TG, VEC>(at(gp, c0));
+      x[k] = load_pack<TX, VEC>(at(xp, c0));
+      if (k + 1 < left) gp += p.gate_rs, xp += p.x_rs;  // behind the last row, that one again
     }
+    gates_of_logarithms<TG, VEC, S>(p, gate);
   }
   const RowSpan span = row_span<S, PACKED>(p, b, r0);
-  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return p.log_gate ? expf(g.value(j)) : g.value(j); };
+  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return LOG16 ? expf(g.value(j)) : g.value(j); };
   auto step = [&](int k, float (&h)[VEC], float (&A)[VEC], int& s) {
     if (span.heads >> k & 1) {
       next_sequence<PACKED>(p, r0 + k, s);
-      load_state<VEC>(p.init, (int64_t)s * C + c0, h);
+      load_state<VEC>(p.init, (int64_t)s * C, c0, h);
     }
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
@@ -443,19 +454,20 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   }
   __syncthreads();
   if (p.ntiles > 1) {
-    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, c0, active, block_c0);
+    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, block_c0);
   } else {
-    if (tid < CH) sm.carry[tid] = 0.f;
+    if (tid < CH) sm.map_h[tid] = 0.f;
+    if (tid == 0) sm.in_group = 1;
     __syncthreads();
   }
 
   wave_carry<VEC>(sm, w, lane, h);
   s = span.first_sequence;
   if (p.states && left > 0 && r0 % kLinChunk == 0 && active) {
-    if (span.heads & 1) load_state<VEC>(p.init, (int64_t)s * C + c0, A);
-    store_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + r0 / kLinChunk) * C + c0, span.heads & 1 ? A : h);
+    if (span.heads & 1) load_state<VEC>(p.init, (int64_t)s * C, c0, A);
+    store_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + r0 / kLinChunk) * C, c0, span.heads & 1 ? A : h);
   }
-  TX* out = static_cast<TX*>(p.out) + b * p.out_bs + c0;
+  TX* out = static_cast<TX*>(p.out) + b * p.out_bs + r0 * p.out_rs;
 #pragma unroll
   for (int k = 0; k < S; k++) forget(gate[k]), forget(x[k]);
 #pragma unroll
@@ -463,19 +475,19 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
     if (span.inside >> k & 1) {
       step(k, h, A, s);
       if (active) {
-        store_pack<TX, VEC>(out + (r0 + k) * p.out_rs, Pack<TX, VEC>::of(h));
-        if (p.final_state && span.ends >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C + c0, h);
+        store_pack<TX, VEC>(at(out + k * p.out_rs, c0), Pack<TX, VEC>::of(h));
+        if (p.final_state && span.ends >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C, c0, h);
       }
     } else if (PACKED && p.clear_outside && k < left && active) {
-      store_pack<TX, VEC>(out + (r0 + k) * p.out_rs, Pack<TX, VEC>{});
+      store_pack<TX, VEC>(at(out + k * p.out_rs, c0), Pack<TX, VEC>{});
     }
   }
   if (p.final_state) {
     if constexpr (PACKED) {
       empty_sequences<VEC>(p, i, p.init, p.final_state, c0, active);
     } else if (p.rows == 0 && w == 0) {
-      load_state<VEC>(p.init, (int64_t)b * C + c0, h);
-      if (active) store_state<VEC>(p.final_state, (int64_t)b * C + c0, h);
+      load_state<VEC>(p.init, (int64_t)b * C, c0, h);
+      if (active) store_state<VEC>(p.final_state, (int64_t)b * C, c0, h);
     }
   }
 }
@@ -485,11 +497,11 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
 // states of its rows are computed again, in 32 bits, from the gates and inputs, which costs no more
 // memory traffic than reading the outputs would and does not differentiate their rounding.
 // ---------------------------------------------------------------------------------------
-template <class TG, class TX, int VEC, bool PACKED>
-__global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs p) {
+template <class TG, class TX, int VEC, bool PACKED, bool LOG16>
+__global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) void linear_scan_backward_kernel(LinArgs p) {
   constexpr int S = kLinChunk / kLinWaves, CH = kWave * VEC, R = kLinChunk;
   __shared__ LinShared<CH> sm;
-  __shared__ float fwd[kLinWaves][CH];
+  __shared__ float fwd[kLinWaves][CH], entering[CH];
   __shared__ int fwd_anew[kLinWaves];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int lw = kLinWaves - 1 - w;
@@ -498,41 +510,43 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs
   take_lin_tile(p, &sm.ticket, i, b, cb);
   const int64_t tile = p.ntiles - 1 - i;
   const int64_t C = p.channels, block_c0 = (int64_t)cb * CH;
-  const int64_t at = block_c0 + lane * VEC;
-  const bool active = at < C;
-  const int64_t c0 = at + VEC > C ? C - VEC : at;
+  const int64_t from = block_c0 + lane * VEC;
+  const bool active = from < C;
+  const uint32_t c0 = (uint32_t)(from + VEC > C ? C - VEC : from);
   const int64_t r0 = tile * R + w * S;
-  const int64_t left = p.rows - r0;
+  const int64_t rows_left = p.rows - r0;
+  const int left = rows_left < 0 ? 0 : rows_left < S ? (int)rows_left : S;  // of this wavefront's S
 
   Pack<TG, VEC> gate[S];
   Pack<TX, VEC> x[S], d[S];
-  float h[VEC], enter[VEC];
+  float h[VEC], enter[VEC] = {};
   if (left > 0) {
-    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + c0;
-    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + c0;
-    const TX* dp = static_cast<const TX*>(p.grad_out) + b * p.grad_bs + c0;
+    const TG* gp = static_cast<const TG*>(p.gate) + b * p.gate_bs + r0 * p.gate_rs;
+    const TX* xp = static_cast<const TX*>(p.x) + b * p.x_bs + r0 * p.x_rs;
+    const TX* dp = static_cast<const TX*>(p.grad_out) + b * p.grad_bs + r0 * p.grad_rs;
 #pragma unroll
     for (int k = 0; k < S; k++) {
-      const int64_t row = k < left ? r0 + k : p.rows - 1;
-      gate[k] = load_pack<TG, VEC>(gp + row * p.gate_rs);
-      x[k] = load_pack<TX, VEC>(xp + row * p.x_rs);
-      d[k] = load_pack<TX, VEC>(dp + row * p.grad_rs);
+      gate[k] = load_pack<TG, VEC>(at(gp, c0));
+      x[k] = load_pack<TX, VEC>(at(xp, c0));
+      d[k] = load_pack<TX, VEC>(at(dp, c0));
+      if (k + 1 < left) gp += p.gate_rs, xp += p.x_rs, dp += p.grad_rs;
     }
-    load_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + tile) * C + c0, enter);
+    gates_of_logarithms<TG, VEC, S>(p, gate);
+    if (w == 0) load_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + tile) * C, c0, enter);
   }
   const RowSpan span = row_span<S, PACKED>(p, b, r0);
-  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return p.log_gate ? expf(g.value(j)) : g.value(j); };
+  auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return LOG16 ? expf(g.value(j)) : g.value(j); };
   // one row of the recurrence, and one of its gradient (c: in the gradient of the state after the row, out that of the one before)
   auto step = [&](int k, float (&hh)[VEC], int& s) {
     if (span.heads >> k & 1) {
       next_sequence<PACKED>(p, r0 + k, s);
-      load_state<VEC>(p.init, (int64_t)s * C + c0, hh);
+      load_state<VEC>(p.init, (int64_t)s * C, c0, hh);
     }
   };
   auto turn = [&](int k, float (&c)[VEC], int& s) {
     if (span.ends >> k & 1) {
       previous_sequence<PACKED>(p, r0 + k, s);
-      load_state<VEC>(p.grad_final, (int64_t)s * C + c0, c);
+      load_state<VEC>(p.grad_final, (int64_t)s * C, c0, c);
     }
   };
   float A[VEC], c[VEC];
@@ -565,6 +579,7 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs
     sm.a[lw][lane * VEC + j] = A[j];
     sm.h[lw][lane * VEC + j] = c[j];
     fwd[w][lane * VEC + j] = h[j];
+    if (w == 0) entering[lane * VEC + j] = enter[j];
   }
   if (lane == 0) {
     sm.anew[lw] = span.ends != 0;
@@ -583,21 +598,25 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs
   }
   __syncthreads();
   if (p.ntiles > 1) {
-    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, c0, active, block_c0);
+    tile_carry<VEC>(sm, p, b, i, p.ntiles, R, block_c0);
   } else {
-    if (tid < CH) sm.carry[tid] = 0.f;
+    if (tid < CH) sm.map_h[tid] = 0.f;
+    if (tid == 0) sm.in_group = 1;
     __syncthreads();
   }
 
+#pragma unroll
+  for (int k = 0; k < S; k++) forget(gate[k]), forget(x[k]), forget(d[k]);
   // states before each row
   int last_anew = -1;
   for (int v = 0; v < w; v++)
     if (fwd_anew[v]) last_anew = v;
+  last_anew = __builtin_amdgcn_readfirstlane(last_anew);
   if (left > 0) {
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
       const int ch = lane * VEC + j;
-      h[j] = last_anew >= 0 ? fwd[last_anew][ch] : enter[j];
+      h[j] = last_anew >= 0 ? fwd[last_anew][ch] : entering[ch];
       for (int v = last_anew + 1; v < w; v++) h[j] = sm.a[kLinWaves - 1 - v][ch] * h[j] + fwd[v][ch];
     }
   }
@@ -615,8 +634,8 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs
     }
   }
   wave_carry<VEC>(sm, lw, lane, c);
-  TG* grad_gate = static_cast<TG*>(p.grad_gate) + b * p.grad_gate_bs + c0;
-  TX* grad_x = static_cast<TX*>(p.out) + b * p.out_bs + c0;
+  TG* grad_gate = static_cast<TG*>(p.grad_gate) + b * p.grad_gate_bs + r0 * p.grad_gate_rs;
+  TX* grad_x = static_cast<TX*>(p.out) + b * p.out_bs + r0 * p.out_rs;
 #pragma unroll
   for (int k = S - 1; k >= 0; k--) {
     if (span.inside >> k & 1) {
@@ -633,82 +652,122 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_backward_kernel(LinArgs
         dg[j] = p.log_gate ? da * a : da;
       }
       if (active) {
-        store_pack<TX, VEC>(grad_x + (r0 + k) * p.out_rs, Pack<TX, VEC>::of(dx));
-        store_pack<TG, VEC>(grad_gate + (r0 + k) * p.grad_gate_rs, Pack<TG, VEC>::of(dg));
-        if (p.final_state && span.heads >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C + c0, c);
+        store_pack<TX, VEC>(at(grad_x + k * p.out_rs, c0), Pack<TX, VEC>::of(dx));
+        store_pack<TG, VEC>(at(grad_gate + k * p.grad_gate_rs, c0), Pack<TG, VEC>::of(dg));
+        if (p.final_state && span.heads >> k & 1) store_state<VEC>(p.final_state, (int64_t)s * C, c0, c);
       }
     } else if (PACKED && p.clear_outside && k < left && active) {
-      store_pack<TX, VEC>(grad_x + (r0 + k) * p.out_rs, Pack<TX, VEC>{});
-      store_pack<TG, VEC>(grad_gate + (r0 + k) * p.grad_gate_rs, Pack<TG, VEC>{});
+      store_pack<TX, VEC>(at(grad_x + k * p.out_rs, c0), Pack<TX, VEC>{});
+      store_pack<TG, VEC>(at(grad_gate + k * p.grad_gate_rs, c0), Pack<TG, VEC>{});
     }
   }
   if (p.final_state) {
     if constexpr (PACKED) {
       empty_sequences<VEC>(p, i, p.grad_final, p.final_state, c0, active);
     } else if (p.rows == 0 && w == 0) {
-      load_state<VEC>(p.grad_final, (int64_t)b * C + c0, h);
-      if (active) store_state<VEC>(p.final_state, (int64_t)b * C + c0, h);
+      load_state<VEC>(p.grad_final, (int64_t)b * C, c0, h);
+      if (active) store_state<VEC>(p.final_state, (int64_t)b * C, c0, h);
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // One token for each of a batch: state[slot] = a state[slot] + x, out = state.  Rows of one slot are
-// taken in their order: the first of them does all, the others leave.
+// taken in their order: the first of them does all, the others leave.  What bounds it is memory; to
+// know whether a row is the first of its slot a workgroup reads all slots, 16 bytes a thread, which is
+// why it takes UNIT vectors of channels a thread where the batch fills the device all the same.
 // ---------------------------------------------------------------------------------------
 constexpr int kStepBlock = 256;
+constexpr int kStepWide = 4;  // vectors a thread takes in a large batch
 
-template <class TG, class TX, int VEC>
+template <class TG, class TX, int UNITS, bool LOG>
 __global__ __launch_bounds__(kStepBlock) void linear_scan_step_kernel(const TG* gate, int64_t gate_rs, const TX* x, int64_t x_rs, TX* out,
                                                                       int64_t out_rs, float* state, int64_t num_slots, const int32_t* slots,
-                                                                      int batch, int64_t C, int ncb, int log_gate) {
-  __shared__ int s_earlier, s_later;
-  const int tid = threadIdx.x, lane = tid % kWave;
+                                                                      int batch, int64_t C, int ncb) {
+  constexpr int VEC = 4;
+  __shared__ int s_found[kStepBlock / kWave];  // bit 0: an earlier row of this slot, bit 1: a later one
+  const int tid = threadIdx.x;
   const int row = (int)(blockIdx.x / (unsigned)ncb), cb = (int)(blockIdx.x % (unsigned)ncb);
-  const int64_t at = ((int64_t)cb * kStepBlock + tid) * VEC;
-  const bool active = at < C;
-  const int64_t c0 = at + VEC > C ? C - VEC : at;
-  const int64_t slot = slots ? slots[row] : row;
+  const int slot = slots ? slots[row] : row;
+  uint32_t c0[UNITS];
+  int n[UNITS];  // channels of each vector; 0: none
+#pragma unroll
+  for (int u = 0; u < UNITS; u++) {
+    const int64_t from = (((int64_t)cb * UNITS + u) * kStepBlock + tid) * VEC;
+    n[u] = C - from >= VEC ? VEC : C - from > 0 ? (int)(C - from) : 0;
+    c0[u] = (uint32_t)from;
+  }
+  auto load = [&](auto* p, int u) {
+    using T = typename std::remove_cv<typename std::remove_pointer<decltype(p)>::type>::type;
+    if (n[u] == VEC) return load_pack<T, VEC>(at(p, c0[u]));
+    return n[u] ? load_part<T, VEC>(at(p, c0[u]), n[u]) : Pack<T, VEC>{};
+  };
+  auto store = [&](auto* p, int u, const auto& v) {
+    if (n[u] == VEC) store_pack(at(p, c0[u]), v);
+    else if (n[u]) store_part(at(p, c0[u]), v, n[u]);
+  };
   if (slot < 0 || slot >= num_slots) {  // a padded row
-    if (active) store_pack<TX, VEC>(out + row * out_rs + c0, Pack<TX, VEC>{});
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) store(out + (int64_t)row * out_rs, u, Pack<TX, VEC>{});
     return;
   }
-  Pack<TG, VEC> g = load_pack<TG, VEC>(gate + row * gate_rs + c0);
-  Pack<TX, VEC> v = load_pack<TX, VEC>(x + row * x_rs + c0);
-  float* sp = state + slot * C + c0;
-  float h[VEC];
-  load_state<VEC>(sp, 0, h);
-  if (slots) {
-    if (tid < kWave) {
-      uint64_t earlier = 0, later = 0;
-      for (int q = lane; q < batch + lane; q += kWave) {
-        const bool same = q < batch && slots[q < batch ? q : batch - 1] == slot;
-        earlier |= __ballot(same && q < row);
-        later |= __ballot(same && q > row);
-      }
-      if (tid == 0) s_earlier = earlier != 0, s_later = later != 0;
-    }
-    __syncthreads();
-    if (s_earlier) return;
+  float* own = state + (int64_t)slot * C;
+  Pack<TG, VEC> g[UNITS];
+  Pack<TX, VEC> v[UNITS];
+  Pack<float, VEC> old[UNITS];
+#pragma unroll
+  for (int u = 0; u < UNITS; u++) {
+    old[u] = load(own, u);
+    g[u] = load(gate + (int64_t)row * gate_rs, u);
+    v[u] = load(x + (int64_t)row * x_rs, u);
   }
+  int found = 0;
+  if (slots) {
+    int mine = 0;
+    auto look = [&](int q, int s) { mine |= s == slot ? (q < row ? 1 : q > row ? 2 : 0) : 0; };
+    for (int q = tid * 4; q < batch; q += kStepBlock * 4) {
+      if (q + 4 <= batch) {
+        const tcd_v4u s = *reinterpret_cast<const tcd_v4u_anywhere*>(slots + q);
+#pragma unroll
+        for (int k = 0; k < 4; k++) look(q + k, (int)s[k]);
+      } else {
+        for (int k = q; k < batch; k++) look(k, slots[k]);
+      }
+    }
+    const uint64_t earlier = __ballot(mine & 1), later = __ballot(mine & 2);
+    if (tid % kWave == 0) s_found[tid / kWave] = (earlier != 0) | (later != 0) << 1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kStepBlock / kWave; w++) found |= s_found[w];
+    if (found & 1) return;
+  }
+  float h[UNITS][VEC];
+#pragma unroll
+  for (int u = 0; u < UNITS; u++)
+#pragma unroll
+    for (int j = 0; j < VEC; j++) h[u][j] = old[u].value(j);
   auto one = [&](int q) {
 #pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      const float a = log_gate ? expf(g.value(j)) : g.value(j);
-      h[j] = a * h[j] + v.value(j);
+    for (int u = 0; u < UNITS; u++) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) h[u][j] = (LOG ? expf(g[u].value(j)) : g[u].value(j)) * h[u][j] + v[u].value(j);
+      store(out + (int64_t)q * out_rs, u, Pack<TX, VEC>::of(h[u]));
     }
-    if (active) store_pack<TX, VEC>(out + q * out_rs + c0, Pack<TX, VEC>::of(h));
   };
   one(row);
-  if (slots && s_later) {
+  if (found & 2) {
     for (int q = row + 1; q < batch; q++) {
       if (slots[q] != slot) continue;
-      g = load_pack<TG, VEC>(gate + q * gate_rs + c0);
-      v = load_pack<TX, VEC>(x + q * x_rs + c0);
+#pragma unroll
+      for (int u = 0; u < UNITS; u++) {
+        g[u] = load(gate + (int64_t)q * gate_rs, u);
+        v[u] = load(x + (int64_t)q * x_rs, u);
+      }
       one(q);
     }
   }
-  if (active) store_state<VEC>(sp, 0, h);
+#pragma unroll
+  for (int u = 0; u < UNITS; u++) store(own, u, Pack<float, VEC>::of(h[u]));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -731,8 +790,8 @@ struct LinPlan {
   size_t tile_at, group_at, super_at, bytes, clear;
 };
 
-inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_rows, bool narrow, LinPlan& l) {
-  l.vec = narrow ? 1 : 4;
+inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_rows, int vec, LinPlan& l) {
+  l.vec = vec;
   const int64_t ncb = ceil_div(channels, (int64_t)kWave * l.vec);
   l.ntiles = rows > 0 ? ceil_div(rows, (int64_t)tile_rows) : 1;
   const double grid = (double)ncb * (double)batch * (double)l.ntiles;
@@ -769,7 +828,7 @@ template <class TG, class TX>
 constexpr int lin_rows_per_wave() { return sizeof(TG) == 2 && sizeof(TX) == 2 ? 16 : 8; }
 
 inline bool valid_shape(int64_t batch, int64_t rows, int64_t channels, int64_t sequences, const void* offsets, int offset_bytes) {
-  if (batch < 0 || rows < 0 || channels < 0 || channels > 0x7fffffff || batch > 0x7fffffff) return false;
+  if (batch < 0 || rows < 0 || channels < 0 || channels > kLinMaxChannels || batch > 0x7fffffff) return false;
   if (offsets || offset_bytes) return batch == 1 && (offset_bytes == 4 || offset_bytes == 8) && sequences >= 0 && sequences < 0x7fffffff;
   return true;
 }
@@ -802,8 +861,7 @@ extern "C" int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const th
     using TX = decltype(tx);
     constexpr int S = lin_rows_per_wave<TG, TX>();
     LinPlan l;
-    const bool narrow = lin_narrow(a->channels, in_place);
-    if (!lin_plan(a->batch, a->rows, a->channels, S * kLinWaves, narrow, l)) return;
+    if (!lin_plan(a->batch, a->rows, a->channels, S * kLinWaves, lin_narrow(a->channels, in_place) ? 1 : 4, l)) return;
     if (temp == nullptr) {
       *temp_bytes = l.bytes;
       rc = hipSuccess;
@@ -835,8 +893,15 @@ extern "C" int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const th
       if (rc != hipSuccess) return;
     }
     const dim3 grid((unsigned)((int64_t)l.ncb * a->batch * l.ntiles));
+    auto launch = [&](auto vec, auto pk, auto log16) {
+      TCD_LAUNCH("linear_scan_kernel", (linear_scan_kernel<TG, TX, decltype(vec)::value, S, decltype(pk)::value, decltype(log16)::value>), grid,
+                 dim3(kLinBlock), s, p);
+    };
     auto go = [&](auto vec, auto pk) {
-      TCD_LAUNCH("linear_scan_kernel", (linear_scan_kernel<TG, TX, decltype(vec)::value, S, decltype(pk)::value>), grid, dim3(kLinBlock), s, p);
+      if constexpr (sizeof(TG) == 2) {
+        if (p.log_gate) return launch(vec, pk, std::true_type{});
+      }
+      launch(vec, pk, std::false_type{});
     };
     using One = std::integral_constant<int, 1>;
     using Four = std::integral_constant<int, 4>;
@@ -869,8 +934,8 @@ extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes,
     using TG = decltype(tg);
     using TX = decltype(tx);
     LinPlan l;
-    const bool narrow = lin_narrow(a->channels, in_place);
-    if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, narrow, l)) return;
+    constexpr int kWide = sizeof(TX) == 4 ? 2 : 4;  // the payload of a lane: three arrays of 8 rows
+    if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, lin_narrow(a->channels, in_place) ? 1 : kWide, l)) return;
     if (temp == nullptr) {
       *temp_bytes = l.bytes;
       rc = hipSuccess;
@@ -907,14 +972,20 @@ extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes,
       if (rc != hipSuccess) return;
     }
     const dim3 grid((unsigned)((int64_t)l.ncb * a->batch * l.ntiles));
+    auto launch = [&](auto vec, auto pk, auto log16) {
+      TCD_LAUNCH("linear_scan_backward_kernel", (linear_scan_backward_kernel<TG, TX, decltype(vec)::value, decltype(pk)::value, decltype(log16)::value>),
+                 grid, dim3(kLinBlock), s, p);
+    };
     auto go = [&](auto vec, auto pk) {
-      TCD_LAUNCH("linear_scan_backward_kernel", (linear_scan_backward_kernel<TG, TX, decltype(vec)::value, decltype(pk)::value>), grid,
-                 dim3(kLinBlock), s, p);
+      if constexpr (sizeof(TG) == 2) {
+        if (p.log_gate) return launch(vec, pk, std::true_type{});
+      }
+      launch(vec, pk, std::false_type{});
     };
     using One = std::integral_constant<int, 1>;
-    using Four = std::integral_constant<int, 4>;
+    using Wide = std::integral_constant<int, kWide>;
     if (l.vec == 1) packed ? go(One{}, std::true_type{}) : go(One{}, std::false_type{});
-    else packed ? go(Four{}, std::true_type{}) : go(Four{}, std::false_type{});
+    else packed ? go(Wide{}, std::true_type{}) : go(Wide{}, std::false_type{});
     rc = hipGetLastError();
   });
   return (int)rc;
@@ -924,7 +995,7 @@ extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int lo
                                              const void* x, int64_t x_row_stride, void* out, int64_t out_row_stride, void* state,
                                              int64_t num_slots, const int32_t* slots, int64_t batch, int64_t channels, void* stream) {
   using namespace tcd;
-  if (batch < 0 || channels < 0 || num_slots < 0 || batch > 0x7fffffff || channels > 0x7fffffff) return hipErrorInvalidValue;
+  if (batch < 0 || channels < 0 || num_slots < 0 || batch > 0x7fffffff || channels > kLinMaxChannels) return hipErrorInvalidValue;
   if (!activation_size(gate_dtype) || !activation_size(x_dtype)) return hipErrorInvalidValue;
   if (!slots && batch > num_slots) return hipErrorInvalidValue;
   hipError_t rc = hipErrorInvalidValue;
@@ -936,19 +1007,22 @@ extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int lo
       return;
     }
     if (!gate || !x || !out || (!state && num_slots > 0)) return;
-    // a vector that repeats channels of its neighbour would read a state that the neighbour has replaced
-    const int vec = channels % 4 != 0 ? 1 : 4;
-    const int64_t ncb = ceil_div(channels, (int64_t)kStepBlock * vec);
+    const int64_t vectors = ceil_div(channels, (int64_t)4), few = ceil_div(vectors, (int64_t)kStepBlock);
+    const int64_t wide = ceil_div(vectors, (int64_t)kStepBlock * kStepWide);
+    const bool many = batch * wide >= 2 * (int64_t)device_cu_count();
+    const int64_t ncb = many ? wide : few;
     if ((double)ncb * (double)batch > 2147483647.0) return;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(ncb * batch));
-    auto go = [&](auto v) {
-      TCD_LAUNCH("linear_scan_step_kernel", (linear_scan_step_kernel<TG, TX, decltype(v)::value>), grid, dim3(kStepBlock), s,
-                 static_cast<const TG*>(gate), gate_row_stride, static_cast<const TX*>(x), x_row_stride, static_cast<TX*>(out), out_row_stride,
-                 static_cast<float*>(state), num_slots, slots, (int)batch, channels, (int)ncb, log_gate != 0);
+    auto go = [&](auto units, auto log) {
+      TCD_LAUNCH("linear_scan_step_kernel", (linear_scan_step_kernel<TG, TX, decltype(units)::value, decltype(log)::value>), grid, dim3(kStepBlock),
+                 s, static_cast<const TG*>(gate), gate_row_stride, static_cast<const TX*>(x), x_row_stride, static_cast<TX*>(out), out_row_stride,
+                 static_cast<float*>(state), num_slots, slots, (int)batch, channels, (int)ncb);
     };
-    if (vec == 1) go(std::integral_constant<int, 1>{});
-    else go(std::integral_constant<int, 4>{});
+    using One = std::integral_constant<int, 1>;
+    using Wide = std::integral_constant<int, kStepWide>;
+    if (many) log_gate ? go(Wide{}, std::true_type{}) : go(Wide{}, std::false_type{});
+    else log_gate ? go(One{}, std::true_type{}) : go(One{}, std::false_type{});
     rc = hipGetLastError();
   });
   return (int)rc;

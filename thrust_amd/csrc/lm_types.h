@@ -90,6 +90,30 @@ __device__ inline void store_pack(T* p, const Pack<T, VEC>& r) {
     else p[0] = bit_cast<T>(r.w[0]);
   }
 }
+// The first n < VEC elements of a pack, one by one: the end of a row whose length is no multiple of VEC.
+template <class T, int VEC>
+__device__ inline Pack<T, VEC> load_part(const T* p, int n) {
+  Pack<T, VEC> r{};
+#pragma unroll
+  for (int j = 0; j < VEC - 1; j++) {
+    if (j < n) {
+      if constexpr (sizeof(T) == 4) r.w[j] = bit_cast<uint32_t>(p[j]);
+      else r.w[j / 2] |= (uint32_t)p[j].bits << 16 * (j & 1);
+    }
+  }
+  return r;
+}
+template <class T, int VEC>
+__device__ inline void store_part(T* p, const Pack<T, VEC>& r, int n) {
+#pragma unroll
+  for (int j = 0; j < VEC - 1; j++) {
+    if (j < n) {
+      if constexpr (sizeof(T) == 4) p[j] = bit_cast<T>(r.w[j]);
+      else p[j].bits = (uint16_t)(r.w[j / 2] >> 16 * (j & 1));
+    }
+  }
+}
+
 // Makes the compiler forget what it derived from a pack: a second pass over packed 16-bit values then
 // converts them again instead of keeping the 32-bit ones of the first in twice as many registers.
 template <class T, int VEC>
