@@ -83,6 +83,11 @@ __device__ inline int64_t offset_at(const LinArgs& p, int64_t j) {
   return p.offsets64 ? static_cast<const int64_t*>(p.offsets)[j] : (int64_t) static_cast<const int32_t*>(p.offsets)[j];
 }
 
+__device__ inline int64_t first_lane(int64_t v) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // The last sequence that begins at or before `row` (not empty if `row` is inside one), or -1.  64 offsets a step.
 __device__ inline int sequence_of(const LinArgs& p, int64_t row) {
   const int lane = lane_id();
@@ -102,62 +107,65 @@ __device__ inline int sequence_of(const LinArgs& p, int64_t row) {
 }
 
 // What a wavefront needs to know of its S rows: which of them are inside a sequence, begin one or end
-// one (bit k: row r0 + k), and the sequence of the first of them.
+// one (bit k: row r0 + k) and the sequence of the first of them.  In begins[l], of the wavefront's own in
+// LDS, the row in which the l-th sequence from that one begins, from r0, in 32 bits, which hold it
+// wherever it matters; a wavefront that sees more than 64 sequences searches.
 struct RowSpan {
   uint32_t inside, heads, ends;
   int first_sequence;
+  int64_t since;  // the row in which the first sequence begins
 };
+constexpr int kFarRow = 1 << 30;
+
+__device__ inline int clamp_sequence(const LinArgs& p, int s) { return s >= p.sequences ? p.sequences - 1 : s < 0 ? 0 : s; }
 
 template <int S, bool PACKED>
-__device__ inline RowSpan row_span(const LinArgs& p, int b, int64_t r0) {
-  RowSpan r{0, 0, 0, b};
+__device__ inline RowSpan row_span(const LinArgs& p, int b, int64_t r0, int* own) {
+  RowSpan r{0, 0, 0, b, 0};
   const int64_t left = p.rows - r0;
   const int n = left <= 0 ? 0 : left < S ? (int)left : S;
   if (n == 0) return r;
-  const uint32_t all = (uint32_t)((uint64_t(1) << n) - 1);
   if constexpr (!PACKED) {
-    r.inside = all;
+    r.inside = (uint32_t)((uint64_t(1) << n) - 1);
     r.heads = r0 == 0;
     r.ends = left <= S ? 1u << (n - 1) : 0u;
   } else {
-    const int64_t begin = offset_at(p, 0);
-    int64_t end = offset_at(p, p.sequences);
-    if (end > p.rows) end = p.rows;
-    const int64_t lo = begin > r0 ? begin - r0 : 0, hi = end - r0 < n ? end - r0 : n;
-    if (lo >= hi) return r;
-    r.inside = (uint32_t)((uint64_t(1) << hi) - 1) & ~(uint32_t)((uint64_t(1) << lo) - 1);
-    int s = sequence_of(p, r0 + lo);
-    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
+    if (p.sequences == 0) return r;
+    const int64_t end = first_lane(offset_at(p, p.sequences)) - r0;  // of the last sequence
+    const int s = clamp_sequence(p, sequence_of(p, r0));
     r.first_sequence = s;
-    if (offset_at(p, s) == r0 + lo) r.heads |= 1u << lo;
-    for (int edges = 0; edges <= S; edges++) {  // each edge ends a sequence and, behind empty ones, begins another
-      const int64_t next = offset_at(p, s + 1);
-      if (next > r0 + hi || next <= r0) break;
-      r.ends |= 1u << (int)(next - r0 - 1);
-      const int after = next < r0 + hi ? sequence_of(p, next) : p.sequences;
-      if (after <= s || after >= p.sequences) break;
-      r.heads |= 1u << (int)(next - r0);
-      s = after;
+    const int hi = end < n ? (int)(end < 0 ? 0 : end) : n;
+    int lo = 0;
+    for (int64_t base = s; base <= p.sequences; base += kWave) {
+      const int64_t j = base + lane_id();
+      const int64_t row = j <= p.sequences ? offset_at(p, j) : INT64_MAX;
+      const int64_t from = row - r0;
+      const int begins = row >= r0 + kFarRow ? kFarRow : from < -1 ? -1 : (int)from;
+      if (base == s) {
+        own[lane_id()] = begins;
+        r.since = first_lane(row);
+        lo = __builtin_amdgcn_readfirstlane(begins) < 0 ? 0 : __builtin_amdgcn_readfirstlane(begins);
+        if (lo >= hi) return r;
+        r.inside = (uint32_t)((uint64_t(1) << hi) - 1) & ~(uint32_t)((uint64_t(1) << lo) - 1);
+      }
+      uint64_t edges = __ballot(begins >= lo && begins <= hi);
+      while (edges) {
+        const int k = __builtin_amdgcn_readlane(begins, __builtin_ctzll(edges));
+        edges &= edges - 1;
+        if (k < hi) r.heads |= 1u << k;
+        if (k > lo) r.ends |= 1u << (k - 1);
+      }
+      if (__builtin_amdgcn_readlane(begins, kWave - 1) > hi) break;
     }
-    r.heads &= r.inside;
-    r.ends &= r.inside;
   }
   return r;
 }
+// the sequence that row r0 + k, which is inside one, belongs to; all lanes of the wavefront call
 template <bool PACKED>
-__device__ inline void next_sequence(const LinArgs& p, int64_t row, int& s) {  // to the one that `row` begins
+__device__ inline void to_sequence(const LinArgs& p, const RowSpan& span, const int* own, int64_t r0, int k, int& s) {
   if constexpr (PACKED) {
-    if (offset_at(p, s + 1) > row) return;
-    s = sequence_of(p, row);
-    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
-  }
-}
-template <bool PACKED>
-__device__ inline void previous_sequence(const LinArgs& p, int64_t row, int& s) {  // to the one that holds `row`
-  if constexpr (PACKED) {
-    if (offset_at(p, s) <= row) return;
-    s = sequence_of(p, row);
-    s = s < 0 ? 0 : s >= p.sequences ? p.sequences - 1 : s;
+    const int n = __popcll(__ballot(own[lane_id()] <= k));
+    s = clamp_sequence(p, n < kWave ? span.first_sequence + n - 1 : sequence_of(p, r0 + k));
   }
 }
 
@@ -167,10 +175,6 @@ template <class T>
 __device__ inline T* at(T* row, uint32_t c) {
   using Byte = typename std::conditional<std::is_const<T>::value, const char, char>::type;
   return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + c * (uint32_t)sizeof(T));
-}
-__device__ inline int64_t first_lane(int64_t v) {
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 template <int VEC>
@@ -393,6 +397,7 @@ template <class TG, class TX, int VEC, int S, bool PACKED, bool LOG16>
 __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   constexpr int CH = kWave * VEC, R = S * kLinWaves;
   __shared__ LinShared<CH> sm;
+  __shared__ int begins[PACKED ? kLinWaves : 1][kWave];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   int64_t i;
   int b, cb;
@@ -407,6 +412,7 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   const int64_t rows_left = p.rows - r0;
   const int left = rows_left < 0 ? 0 : rows_left < S ? (int)rows_left : S;  // of this wavefront's S
 
+  const RowSpan span = row_span<S, PACKED>(p, b, r0, begins[PACKED ? w : 0]);  // before the loads of rows: a load that follows them waits for them
   Pack<TG, VEC> gate[S];
   Pack<TX, VEC> x[S];
   if (left > 0) {
@@ -420,11 +426,10 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
     }
     gates_of_logarithms<TG, VEC, S>(p, gate);
   }
-  const RowSpan span = row_span<S, PACKED>(p, b, r0);
   auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return LOG16 ? expf(g.value(j)) : g.value(j); };
   auto step = [&](int k, float (&h)[VEC], float (&A)[VEC], int& s) {
     if (span.heads >> k & 1) {
-      next_sequence<PACKED>(p, r0 + k, s);
+      to_sequence<PACKED>(p, span, begins[PACKED ? w : 0], r0, k, s);
       load_state<VEC>(p.init, (int64_t)s * C, c0, h);
     }
 #pragma unroll
@@ -449,7 +454,7 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   if (lane == 0) sm.anew[w] = span.heads != 0;
   if (w == 0) {
     int64_t since = -1;
-    if (!(span.heads & 1) && (span.inside & 1)) since = PACKED ? offset_at(p, span.first_sequence) : 0;
+    if (!(span.heads & 1) && (span.inside & 1)) since = PACKED ? span.since : 0;
     if (lane == 0) sm.since = since < 0 || since > r0 ? -1 : since;
   }
   __syncthreads();
@@ -501,6 +506,7 @@ template <class TG, class TX, int VEC, bool PACKED, bool LOG16>
 __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) void linear_scan_backward_kernel(LinArgs p) {
   constexpr int S = kLinChunk / kLinWaves, CH = kWave * VEC, R = kLinChunk;
   __shared__ LinShared<CH> sm;
+  __shared__ int begins[PACKED ? kLinWaves : 1][kWave];
   __shared__ float fwd[kLinWaves][CH], entering[CH];
   __shared__ int fwd_anew[kLinWaves];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
@@ -517,6 +523,7 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
   const int64_t rows_left = p.rows - r0;
   const int left = rows_left < 0 ? 0 : rows_left < S ? (int)rows_left : S;  // of this wavefront's S
 
+  const RowSpan span = row_span<S, PACKED>(p, b, r0, begins[PACKED ? w : 0]);  // before the loads of rows: a load that follows them waits for them
   Pack<TG, VEC> gate[S];
   Pack<TX, VEC> x[S], d[S];
   float h[VEC], enter[VEC] = {};
@@ -534,18 +541,17 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
     gates_of_logarithms<TG, VEC, S>(p, gate);
     if (w == 0) load_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + tile) * C, c0, enter);
   }
-  const RowSpan span = row_span<S, PACKED>(p, b, r0);
   auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return LOG16 ? expf(g.value(j)) : g.value(j); };
   // one row of the recurrence, and one of its gradient (c: in the gradient of the state after the row, out that of the one before)
   auto step = [&](int k, float (&hh)[VEC], int& s) {
     if (span.heads >> k & 1) {
-      next_sequence<PACKED>(p, r0 + k, s);
+      to_sequence<PACKED>(p, span, begins[PACKED ? w : 0], r0, k, s);
       load_state<VEC>(p.init, (int64_t)s * C, c0, hh);
     }
   };
   auto turn = [&](int k, float (&c)[VEC], int& s) {
     if (span.ends >> k & 1) {
-      previous_sequence<PACKED>(p, r0 + k, s);
+      to_sequence<PACKED>(p, span, begins[PACKED ? w : 0], r0, k, s);
       load_state<VEC>(p.grad_final, (int64_t)s * C, c0, c);
     }
   };
@@ -640,7 +646,6 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
   for (int k = S - 1; k >= 0; k--) {
     if (span.inside >> k & 1) {
       turn(k, c, s);
-      previous_sequence<PACKED>(p, r0 + k, s);
       float dg[VEC], dx[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; j++) {
@@ -651,6 +656,7 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
         dx[j] = g;
         dg[j] = p.log_gate ? da * a : da;
       }
+      if (span.heads >> k & 1) to_sequence<PACKED>(p, span, begins[PACKED ? w : 0], r0, k, s);
       if (active) {
         store_pack<TX, VEC>(at(grad_x + k * p.out_rs, c0), Pack<TX, VEC>::of(dx));
         store_pack<TG, VEC>(at(grad_gate + k * p.grad_gate_rs, c0), Pack<TG, VEC>::of(dg));
