@@ -18,7 +18,7 @@ if EMULATED:
     def _cpu(*tensors):
         return torch.device("cpu")
 
-    def _empty(shape, dtype, device):
+    def _empty(like, shape, dtype):
         if os.environ.get("THRUST_CDNA4_EMULATED_GUARD") != "1":
             return torch.empty(shape, dtype=dtype)
         two = dtype in (torch.float16, torch.bfloat16)
@@ -26,6 +26,7 @@ if EMULATED:
 
     device.need_device = _cpu
     device.current = lambda d: contextlib.nullcontext()
+    device.is_current = lambda d: True
     device.stream = lambda d: ctypes.c_void_p(0)
     device.empty = _empty
 

@@ -136,6 +136,8 @@ def any_device(monkeypatch):
     """The checks that come after the device's, on host tensors: nothing may be launched."""
     monkeypatch.setattr(device, "need_device", lambda *t: torch.device("cpu"))
     monkeypatch.setattr(device, "current", lambda d: pytest.fail("not refused"))
+    monkeypatch.setattr(device, "is_current", lambda d: pytest.fail("not refused"))
+    monkeypatch.setattr(device, "stream", lambda d: 0)
 
 
 Z = torch.zeros

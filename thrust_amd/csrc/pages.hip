@@ -18,6 +18,11 @@ constexpr int kPageSweep = kPageBlock * kPagesPerThread;  // counts that a workg
 constexpr int kCopyUnit = kPageBlock * 16 * 4;            // bytes that a workgroup copies in one go
 constexpr int kMaxSpans = 8192;
 constexpr int kRequestWaves = kPageBlock / kWave;
+// A cache of this size with this many requests is planned by one workgroup of 16 wavefronts: a launch
+// costs the host about 3 us and the device 2 us, the loops over pages and requests less than that.
+constexpr int kSmallBlock = 1024;
+constexpr int kSmallPages = kSmallBlock * kPagesPerThread;
+constexpr int kSmallRequests = 4 * kSmallBlock / kWave;
 
 struct PageCache {
   const uint64_t* pools;
@@ -34,6 +39,7 @@ struct PageTemp {
   int32_t* span_free;  // free pages of each span
   int32_t* need;       // pages a request wants; -1: refused
   int64_t* start;      // pages wanted by the requests before it
+  int32_t* copied;     // resize: the page that a growing sequence gets a copy of; -1: none
   int32_t* free_list;  // free pages, ascending; a compaction's holes
   int32_t* movers;     // a compaction's pages that move, descending, and their counts
   int32_t* mover_refs;
@@ -53,12 +59,14 @@ __device__ inline void add_count(const PageCache& c, int q, int v) { atomicAdd(r
 // ---------------------------------------------------------------------------------------
 // Sums over the workgroup
 // ---------------------------------------------------------------------------------------
+template <int BLOCK>
 struct BlockSum {
-  int64_t wave_total[kRequestWaves];
+  static constexpr int kThreads = BLOCK;
+  int64_t wave_total[BLOCK / kWave];
 };
 // exclusive prefix of v over the threads, and the total
-template <class T>
-__device__ inline T block_exclusive(BlockSum& sm, T v, T& total) {
+template <int BLOCK, class T>
+__device__ inline T block_exclusive(BlockSum<BLOCK>& sm, T v, T& total) {
   const int w = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const T incl = wave_inclusive_scan(v, T(0), [](T a, T b) { return a + b; });
   __syncthreads();  // the last call's totals have been read
@@ -67,16 +75,17 @@ __device__ inline T block_exclusive(BlockSum& sm, T v, T& total) {
   T before = 0;
   total = 0;
 #pragma unroll
-  for (int k = 0; k < kRequestWaves; k++) {
+  for (int k = 0; k < BLOCK / kWave; k++) {
     if (k < w) before += (T)sm.wave_total[k];
     total += (T)sm.wave_total[k];
   }
   return before + incl - v;
 }
 // the sum of the positive ones of n values, the same in all threads
-__device__ inline int64_t block_sum(BlockSum& sm, const int32_t* v, int64_t n) {
+template <int BLOCK>
+__device__ inline int64_t block_sum(BlockSum<BLOCK>& sm, const int32_t* v, int64_t n) {
   int64_t mine = 0, total;
-  for (int64_t i = threadIdx.x; i < n; i += kPageBlock) mine += v[i] > 0 ? v[i] : 0;
+  for (int64_t i = threadIdx.x; i < n; i += BLOCK) mine += v[i] > 0 ? v[i] : 0;
   block_exclusive(sm, mine, total);
   return total;
 }
@@ -85,7 +94,7 @@ __device__ inline int64_t block_sum(BlockSum& sm, const int32_t* v, int64_t n) {
 // Free pages
 // ---------------------------------------------------------------------------------------
 __device__ inline void tally_span(const PageCache& c, const PageTemp& t, int span) {
-  __shared__ BlockSum sm;
+  __shared__ BlockSum<kPageBlock> sm;
   const int64_t begin = (int64_t)span * t.span;
   const int64_t end = begin + t.span < c.num_pages ? begin + t.span : c.num_pages;
   int mine = 0;
@@ -95,12 +104,12 @@ __device__ inline void tally_span(const PageCache& c, const PageTemp& t, int spa
   if (threadIdx.x == 0) t.span_free[span] = total;
 }
 
-// f(q, count, free pages before q) for every page of a span, in all threads of the workgroup
-template <class F>
-__device__ inline void sweep_span(const PageCache& c, const PageTemp& t, BlockSum& sm, int span, int64_t before, F f) {
+// f(q, count, free pages before q) for every page of a span, by the whole workgroup; the free pages up to its end
+template <int BLOCK, class F>
+__device__ inline int64_t sweep_span(const PageCache& c, const PageTemp& t, BlockSum<BLOCK>& sm, int span, int64_t before, F f) {
   const int64_t begin = (int64_t)span * t.span;
   const int64_t end = begin + t.span < c.num_pages ? begin + t.span : c.num_pages;
-  for (int64_t at = begin; at < end; at += kPageSweep) {
+  for (int64_t at = begin; at < end; at += BLOCK * kPagesPerThread) {
     int n[kPagesPerThread];
     const int64_t q0 = at + (int64_t)threadIdx.x * kPagesPerThread;
     int mine = 0;
@@ -118,17 +127,31 @@ __device__ inline void sweep_span(const PageCache& c, const PageTemp& t, BlockSu
     }
     before += total;
   }
+  return before;
 }
 
 // ---------------------------------------------------------------------------------------
 // Requests
 // ---------------------------------------------------------------------------------------
-// whether an earlier request names the same sequence (all lanes of a wavefront ask for the same one)
+// whether an earlier request names the same sequence (all lanes of a wavefront ask for the same one):
+// 16 bytes a lane and four of them in flight, 1024 requests a trip
 __device__ inline bool named_before(const int32_t* named, int64_t i, int s) {
   bool found = false;
-  for (int64_t q0 = 0; q0 < i; q0 += kWave) {
-    const int64_t q = q0 + lane_id();
-    found = found || (q < i && named[q] == s);
+  int64_t q0 = (int64_t)lane_id() * 4;
+  for (; q0 + 3 * 4 * kWave + 4 <= i; q0 += 4 * 4 * kWave) {
+    tcd_v4u v[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const tcd_v4u_anywhere*>(named + q0 + k * 4 * kWave);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      found = found || (int)v[k][0] == s || (int)v[k][1] == s || (int)v[k][2] == s || (int)v[k][3] == s;
+  }
+  for (; q0 < i; q0 += 4 * kWave) {
+    int v[4];  // behind the end, the last one again, which is an earlier one too
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = named[q0 + k < i ? q0 + k : i - 1];
+#pragma unroll
+    for (int k = 0; k < 4; k++) found = found || v[k] == s;
   }
   return __ballot(found) != 0;
 }
@@ -144,11 +167,9 @@ struct Requests {
   uint8_t* done;
 };
 
-// Shrinks and frees.  need[i] = 0, or -1 where the request is refused.
-__global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, PageTemp t, Requests r) {
+// Shrinks and frees, a wavefront for a request.  need[i] = 0, or -1 where the request is refused.
+__device__ inline void shrink(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
   const int lane = lane_id();
-  const int64_t i = (int64_t)blockIdx.x * kRequestWaves + threadIdx.x / kWave;
-  if (i >= r.n) return;
   const int s = r.named[i];
   const int64_t want = r.first ? r.first[i] : 0;
   bool ok = s >= 0 && s < c.num_sequences && want >= 0 && want <= (int64_t)c.max_pages * c.page_size;
@@ -168,6 +189,10 @@ __global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, P
   }
   if (lane == 0) c.lengths[s] = (int)want;
 }
+__global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, PageTemp t, Requests r) {
+  const int64_t i = (int64_t)blockIdx.x * kRequestWaves + threadIdx.x / kWave;
+  if (i < r.n) shrink(c, t, r, i);
+}
 
 // the last page of a growing sequence when others name it too and something of it is free
 __device__ inline int page_to_copy(const PageCache& c, int s, int old, int want) {
@@ -176,18 +201,16 @@ __device__ inline int page_to_copy(const PageCache& c, int s, int old, int want)
   return is_page(c, q) && c.refs[q] > 1 ? q : -1;
 }
 
-// Tallies the free pages and what each request wants.
-__global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, PageTemp t, Requests r) {
-  if ((int)blockIdx.x < t.spans) return tally_span(c, t, (int)blockIdx.x);
-  if (r.kind == kResize) {
-    const int64_t i = (int64_t)(blockIdx.x - t.spans) * kPageBlock + threadIdx.x;
-    if (i >= r.n || t.need[i] < 0) return;
-    const int s = r.named[i], old = clamped_length(c, s), want = r.first[i];
-    t.need[i] = want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (page_to_copy(c, s, old, want) >= 0);
-    return;
-  }
-  const int64_t i = (int64_t)(blockIdx.x - t.spans) * kRequestWaves + threadIdx.x / kWave;
-  if (i >= r.n) return;
+// What a resize wants, a thread for a request.
+__device__ inline void want_resize(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
+  if (t.need[i] < 0) return;
+  const int s = r.named[i], old = clamped_length(c, s), want = r.first[i];
+  const int q = page_to_copy(c, s, old, want);
+  t.copied[i] = q;
+  t.need[i] = want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (q >= 0);
+}
+// What a fork wants, a wavefront for a request.
+__device__ inline void want_fork(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
   const int parent = r.first[i], child = r.named[i];
   bool ok = parent >= 0 && parent < c.num_sequences && child >= 0 && child < c.num_sequences;
   if (ok) ok = c.lengths[child] == 0 && !named_before(r.named, i, child) && !named_anywhere(r.first, r.n, child);
@@ -199,9 +222,22 @@ __global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, Pa
   if (lane_id() == 0) t.need[i] = need;
 }
 
+// Tallies the free pages and what each request wants.
+__global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, PageTemp t, Requests r) {
+  if ((int)blockIdx.x < t.spans) return tally_span(c, t, (int)blockIdx.x);
+  const int64_t block = blockIdx.x - t.spans;
+  if (r.kind == kResize) {
+    const int64_t i = block * kPageBlock + threadIdx.x;
+    if (i < r.n) want_resize(c, t, r, i);
+  } else {
+    const int64_t i = block * kRequestWaves + threadIdx.x / kWave;
+    if (i < r.n) want_fork(c, t, r, i);
+  }
+}
+
 // Lists the free pages, as many as are wanted, and adds up the requests.
 __global__ __launch_bounds__(kPageBlock) void pages_list_kernel(PageCache c, PageTemp t, int64_t n) {
-  __shared__ BlockSum sm;
+  __shared__ BlockSum<kPageBlock> sm;
   if ((int)blockIdx.x == t.spans) {
     int64_t sum = 0;
     for (int64_t at = 0; at < n; at += kPageBlock) {
@@ -222,6 +258,30 @@ __global__ __launch_bounds__(kPageBlock) void pages_list_kernel(PageCache c, Pag
   sweep_span(c, t, sm, (int)blockIdx.x, before, [&](int64_t q, int count, int64_t rank) {
     if (count == 0 && rank < wanted) t.free_list[rank] = (int)q;
   });
+}
+
+// All of that for a small cache and few requests, in one workgroup instead of two or three launches.
+__global__ __launch_bounds__(kSmallBlock) void pages_plan_small_kernel(PageCache c, PageTemp t, Requests r) {
+  __shared__ BlockSum<kSmallBlock> sm;
+  const int w = threadIdx.x / kWave, i = threadIdx.x;
+  if (r.kind == kResize) {
+    for (int64_t k = w; k < r.n; k += kSmallBlock / kWave) shrink(c, t, r, k);
+    __threadfence();  // lengths, counts and needs are read by other wavefronts below
+    __syncthreads();
+    if (i < r.n) want_resize(c, t, r, i);
+  } else {
+    for (int64_t k = w; k < r.n; k += kSmallBlock / kWave) want_fork(c, t, r, k);
+    __threadfence();
+    __syncthreads();
+  }
+  const int64_t need = i < r.n && t.need[i] > 0 ? t.need[i] : 0;
+  int64_t wanted;
+  const int64_t start = block_exclusive(sm, need, wanted);
+  if (i < r.n) t.start[i] = start;
+  const int64_t free = sweep_span(c, t, sm, 0, 0, [&](int64_t q, int count, int64_t rank) {
+    if (count == 0 && rank < wanted) t.free_list[rank] = (int)q;
+  });
+  if (i == 0) t.head[1] = free;
 }
 
 // bytes [at, at + n) of a page, n <= kCopyUnit, by the whole workgroup
@@ -269,29 +329,33 @@ __global__ __launch_bounds__(kPageBlock) void pages_serve_kernel(PageCache c, Pa
   const int s = r.named[i];
   int32_t* row = c.tables + (int64_t)s * c.max_pages;
   const int64_t units = (c.page_bytes + kCopyUnit - 1) / kCopyUnit;
-
   if (r.kind == kResize) {
-    const int want = r.first[i], old = clamped_length(c, s);
-    if (want <= old) return;
-    const int had = pages_of(c, old), have = pages_of(c, want), last = old / c.page_size;
-    const int own = need - (have - had);  // 1: a copy of the last page was asked for
-    const int q = own ? row[last] : -1;
-    __syncthreads();  // all threads have the old length and entry
-    if (own) {
-      for (int64_t u = 0; u < units * c.num_pools; u++) copy_page_unit(c, (int)(u / units), q, mine[0], u % units);
+    const int want = r.first[i];
+    if (need == 0) {  // it shrank before, or grows within its last page
+      if (piece == 0 && threadIdx.x == 0 && want > clamped_length(c, s)) c.lengths[s] = want;
+      return;
     }
-    for (int j = had + (int)threadIdx.x; j < have; j += kPageBlock) {
-      const int page = mine[own + j - had];
-      row[j] = page;
-      c.refs[page] = 1;
-    }
-    if (threadIdx.x == 0) {
-      if (own) {
-        row[last] = mine[0];
-        c.refs[mine[0]] = 1;
-        add_count(c, q, -1);
+    const int q = t.copied[i], own = q >= 0;
+    if (piece == 0) {
+      // its pages from the first one behind the old length: `had` comes from what is wanted, not from the
+      // length, which a thread of this workgroup may have replaced
+      const int have = pages_of(c, want), had = have - (need - own);
+      for (int j = had + (int)threadIdx.x; j < have; j += kPageBlock) {
+        const int page = mine[own + j - had];
+        row[j] = page;
+        c.refs[page] = 1;
       }
-      c.lengths[s] = want;
+      if (threadIdx.x == 0) {
+        if (own) {
+          row[had - 1] = mine[0];
+          c.refs[mine[0]] = 1;
+          add_count(c, q, -1);
+        }
+        c.lengths[s] = want;
+      }
+    }
+    if (own) {
+      for (int64_t u = piece; u < units * c.num_pools; u += pieces) copy_page_unit(c, (int)(u / units), q, mine[0], u % units);
     }
     return;
   }
@@ -324,15 +388,14 @@ __global__ __launch_bounds__(kPageBlock) void pages_serve_kernel(PageCache c, Pa
 // ---------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kPageBlock) void pages_tally_only_kernel(PageCache c, PageTemp t) { tally_span(c, t, (int)blockIdx.x); }
 
-__global__ __launch_bounds__(kPageBlock) void pages_rank_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
-  __shared__ BlockSum sm;
-  const int64_t before = block_sum(sm, t.span_free, blockIdx.x);
-  const int64_t live = c.num_pages - block_sum(sm, t.span_free, t.spans);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+template <int BLOCK>
+__device__ inline void rank_span(const PageCache& c, const PageTemp& t, BlockSum<BLOCK>& sm, int span, int64_t before, int64_t live, int32_t* refs_out,
+                                 int32_t* live_out) {
+  if (span == 0 && threadIdx.x == 0) {
     *live_out = (int)live;
     if (live == c.num_pages) t.head[0] = 0;
   }
-  sweep_span(c, t, sm, (int)blockIdx.x, before, [&](int64_t q, int count, int64_t rank) {
+  sweep_span(c, t, sm, span, before, [&](int64_t q, int count, int64_t rank) {
     if (q == live) t.head[0] = rank;  // holes below
     if (q < live) {
       if (count == 0) t.free_list[rank] = (int)q;
@@ -348,6 +411,20 @@ __global__ __launch_bounds__(kPageBlock) void pages_rank_kernel(PageCache c, Pag
       refs_out[q] = 0;
     }
   });
+}
+__global__ __launch_bounds__(kPageBlock) void pages_rank_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
+  __shared__ BlockSum<kPageBlock> sm;
+  const int64_t before = block_sum(sm, t.span_free, blockIdx.x);
+  const int64_t live = c.num_pages - block_sum(sm, t.span_free, t.spans);
+  rank_span(c, t, sm, (int)blockIdx.x, before, live, refs_out, live_out);
+}
+// The same for a small cache, in one workgroup that needs no tally of spans.
+__global__ __launch_bounds__(kSmallBlock) void pages_rank_small_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
+  __shared__ BlockSum<kSmallBlock> sm;
+  int used = 0, live;
+  for (int q = threadIdx.x; q < c.num_pages; q += kSmallBlock) used += c.refs[q] != 0;
+  block_exclusive(sm, used, live);
+  rank_span(c, t, sm, 0, 0, live, refs_out, live_out);
 }
 
 __global__ __launch_bounds__(kPageBlock) void pages_move_kernel(PageCache c, PageTemp t, int32_t* tables_out, int32_t* refs_out,
@@ -407,6 +484,7 @@ static size_t page_temp(const PageCache& c, int64_t n, bool compact, void* temp,
   t.span_free = reinterpret_cast<int32_t*>(take((size_t)t.spans * 4));
   t.need = reinterpret_cast<int32_t*>(take((size_t)n * 4));
   t.start = reinterpret_cast<int64_t*>(take((size_t)n * 8));
+  t.copied = reinterpret_cast<int32_t*>(take((size_t)n * 4));
   t.free_list = reinterpret_cast<int32_t*>(take((size_t)c.num_pages * 4));
   t.movers = t.mover_refs = t.place = nullptr;
   if (compact) {
@@ -417,19 +495,35 @@ static size_t page_temp(const PageCache& c, int64_t n, bool compact, void* temp,
   return at;
 }
 
-static hipError_t serve(const PageCache& c, const PageTemp& t, const Requests& r, hipStream_t s) {
+static hipError_t grant(const PageCache& c, const PageTemp& t, const Requests& r, hipStream_t s) {
+  // enough workgroups to fill the device, none without a unit to copy; a resize copies a page at most, and rarely
+  const int64_t units = ceil_div(c.page_bytes, (int64_t)kCopyUnit) * c.num_pools * (r.kind == kFork ? c.max_pages : 1);
+  int64_t pieces = ceil_div((int64_t)device_cu_count() * (r.kind == kResize ? 2 : 16), r.n);
+  if (pieces > units) pieces = units;
+  if (pieces < 1) pieces = 1;
+  TCD_LAUNCH("pages_serve_kernel", pages_serve_kernel, dim3((unsigned)(r.n * pieces)), dim3(kPageBlock), s, c, t, r, (int)pieces);
+  return hipGetLastError();
+}
+
+// one span for a small cache
+static bool small_cache(const PageCache& c, PageTemp& t) {
+  if (c.num_pages > kSmallPages) return false;
+  t.span = kSmallPages;
+  t.spans = 1;
+  return true;
+}
+
+static hipError_t serve(const PageCache& c, PageTemp t, const Requests& r, hipStream_t s) {
+  if (r.n <= kSmallRequests && small_cache(c, t)) {
+    TCD_LAUNCH("pages_plan_small_kernel", pages_plan_small_kernel, dim3(1), dim3(kSmallBlock), s, c, t, r);
+    return grant(c, t, r, s);
+  }
+  if (r.kind == kResize)
+    TCD_LAUNCH("pages_shrink_kernel", pages_shrink_kernel, dim3((unsigned)ceil_div(r.n, (int64_t)kRequestWaves)), dim3(kPageBlock), s, c, t, r);
   const int64_t request_blocks = r.kind == kResize ? ceil_div(r.n, (int64_t)kPageBlock) : ceil_div(r.n, (int64_t)kRequestWaves);
   TCD_LAUNCH("pages_tally_kernel", pages_tally_kernel, dim3((unsigned)(t.spans + request_blocks)), dim3(kPageBlock), s, c, t, r);
   TCD_LAUNCH("pages_list_kernel", pages_list_kernel, dim3((unsigned)t.spans + 1u), dim3(kPageBlock), s, c, t, r.n);
-  int64_t pieces = 1;
-  if (r.kind != kResize) {  // enough workgroups to fill the device, none without a unit to copy
-    const int64_t units = ceil_div(c.page_bytes, (int64_t)kCopyUnit) * c.num_pools * (r.kind == kForkShared ? 1 : c.max_pages);
-    pieces = ceil_div((int64_t)device_cu_count() * 16, r.n);
-    if (pieces > units) pieces = units;
-    if (pieces < 1) pieces = 1;
-  }
-  TCD_LAUNCH("pages_serve_kernel", pages_serve_kernel, dim3((unsigned)(r.n * pieces)), dim3(kPageBlock), s, c, t, r, (int)pieces);
-  return hipGetLastError();
+  return grant(c, t, r, s);
 }
 
 }  // namespace tcd
@@ -465,7 +559,6 @@ extern "C" int thrust_cdna4_pages_resize(void* temp, size_t* temp_bytes, const t
   if (*temp_bytes < bytes || !sequences || !lengths || !done || !cache_usable(c)) return hipErrorInvalidValue;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Requests r{lengths, sequences, n, kResize, done};
-  TCD_LAUNCH("pages_shrink_kernel", pages_shrink_kernel, dim3((unsigned)ceil_div(n, (int64_t)kRequestWaves)), dim3(kPageBlock), s, c, t, r);
   return (int)serve(c, t, r, s);
 }
 
@@ -501,6 +594,8 @@ extern "C" int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const 
     if (e != hipSuccess) return (int)e;
     e = zero_async(t.head, 16, s);
     if (e != hipSuccess) return (int)e;
+  } else if (small_cache(c, t)) {
+    TCD_LAUNCH("pages_rank_small_kernel", pages_rank_small_kernel, dim3(1), dim3(kSmallBlock), s, c, t, refs_out, live_out);
   } else {
     TCD_LAUNCH("pages_tally_only_kernel", pages_tally_only_kernel, dim3((unsigned)t.spans), dim3(kPageBlock), s, c, t);
     TCD_LAUNCH("pages_rank_kernel", pages_rank_kernel, dim3((unsigned)t.spans), dim3(kPageBlock), s, c, t, refs_out, live_out);

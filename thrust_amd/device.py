@@ -1,35 +1,44 @@
-"""Where the calls on torch tensors run: the tensors' device, torch's current stream on it."""
+"""Where the calls on torch tensors run: the tensors' device, torch's current stream on it.
+
+A call's own time on the host is most of a small call's time: nothing here builds a Python object that
+it can do without."""
 import contextlib
-import ctypes
 
 import torch
+
+_HERE = contextlib.nullcontext()
 
 
 def need_device(*tensors):
     """The one device that all of the tensors (None: left out) are on."""
-    device = None
+    first = None
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("device tensors required: there is no CPU path")
-        if device is not None and t.device != device:
-            raise ValueError("tensors on different devices")
-        device = t.device
-    return device
+        if t is not None:
+            if not t.is_cuda:
+                raise ValueError("device tensors required: there is no CPU path")
+            if first is None:
+                first = t
+            elif t.get_device() != first.get_device():
+                raise ValueError("tensors on different devices")
+    return None if first is None else first.device
+
+
+def is_current(device):
+    return device.index == torch.cuda.current_device()
 
 
 def current(device):
     """A context in which `device` is the current one."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if is_current(device) else torch.cuda.device(device)
 
 
 def stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def empty(shape, dtype, device):
-    return torch.empty(shape, dtype=dtype, device=device)
+def empty(like, shape, dtype):
+    """Uninitialised, on the device of `like`."""
+    return like.new_empty(shape, dtype=dtype)
 
 
 def pointer(t):
@@ -38,5 +47,6 @@ def pointer(t):
 
 def no_autograd(*tensors):
     """These calls are no nodes of torch's graph: a tensor that wants its gradient is not dropped in silence."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("no automatic differentiation: call under torch.no_grad(), with linear_scan_backward as the gradient")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("no automatic differentiation: call under torch.no_grad(), with linear_scan_backward as the gradient")

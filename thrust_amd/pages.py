@@ -50,7 +50,7 @@ class PageCache:
 
     def _array(self, given, shape, value, what):
         if given is None:
-            return dev.empty(shape, torch.int32, self.device).fill_(value)
+            return dev.empty(self.pools[0], shape, torch.int32).fill_(value)
         if given.dtype != torch.int32 or given.shape != shape or not given.is_contiguous():
             raise ValueError(f"{what} must be int32 {list(shape)}, contiguous")
         return given
@@ -72,7 +72,7 @@ class PageCache:
             if len(self._sizes) > 256:
                 self._sizes.clear()
             self._sizes[key] = nbytes
-        return dev.empty((nbytes.value,), torch.uint8, self.device), ctypes.byref(nbytes)
+        return dev.empty(self.refs, (nbytes.value,), torch.uint8), ctypes.byref(nbytes)
 
     def resize(self, sequences, lengths):
         """sequences[i] gets the length lengths[i] (int32 tensors).  Pages given up are there for the
@@ -81,7 +81,7 @@ class PageCache:
         before, a length out of range, not enough free pages), which changes nothing of the sequence."""
         n = self._requests(sequences, lengths)
         L = capi.lib()
-        done = dev.empty((n,), torch.bool, self.device)
+        done = dev.empty(self.refs, (n,), torch.bool)
         with dev.current(self.device):
             temp, nbytes = self._temp(L.thrust_cdna4_pages_resize, ("pages_resize", n), None, None, n, None)
             capi.check(L.thrust_cdna4_pages_resize(temp.data_ptr(), nbytes, self._ref, sequences.data_ptr(), lengths.data_ptr(), n,
@@ -101,7 +101,7 @@ class PageCache:
         that is not empty, a parent or named before, not enough free pages)."""
         n = self._requests(parents, children)
         L = capi.lib()
-        done = dev.empty((n,), torch.bool, self.device)
+        done = dev.empty(self.refs, (n,), torch.bool)
         with dev.current(self.device):
             temp, nbytes = self._temp(L.thrust_cdna4_pages_fork, ("pages_fork", n), None, None, n, 0, None)
             capi.check(L.thrust_cdna4_pages_fork(temp.data_ptr(), nbytes, self._ref, parents.data_ptr(), children.data_ptr(), n, bool(share),
@@ -119,7 +119,7 @@ class PageCache:
         tables = self.tables if tables is None else self._array(tables, self.tables.shape, None, "tables")
         refs = self.refs if refs is None else self._array(refs, self.refs.shape, None, "refs")
         L = capi.lib()
-        live = dev.empty((1,), torch.int32, self.device)
+        live = dev.empty(self.refs, (1,), torch.int32)
         with dev.current(self.device):
             temp, nbytes = self._temp(L.thrust_cdna4_pages_compact, ("pages_compact",), None, None, None)
             capi.check(L.thrust_cdna4_pages_compact(temp.data_ptr(), nbytes, self._ref, tables.data_ptr(), refs.data_ptr(), live.data_ptr(),

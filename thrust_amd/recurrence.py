@@ -72,12 +72,12 @@ def _strided(fields, name, t, shape):
     fields[name + "_batch_stride"], fields[name + "_row_stride"] = _rows(t, shape, name)
 
 
-def _run(entry, args, device, what):
+def _run(entry, args, device, x, what):
     with dev.current(device):
         nbytes = ctypes.c_size_t(0)
         stream = dev.stream(device)
-        capi.check(entry(None, ctypes.byref(nbytes), ctypes.byref(args), stream), what + "(size)")
-        temp = dev.empty((nbytes.value,), torch.uint8, device)
+        capi.check(entry(None, ctypes.byref(nbytes), ctypes.byref(args), stream), what)
+        temp = dev.empty(x, (nbytes.value,), torch.uint8)
         capi.check(entry(temp.data_ptr(), ctypes.byref(nbytes), ctypes.byref(args), stream), what)
 
 
@@ -92,7 +92,7 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     _state(init, sequences, x.shape[-1], "init")
     fields["clear_outside"] = out is None
     if out is None:
-        out = dev.empty(x.shape, x.dtype, device)
+        out = dev.empty(x, x.shape, x.dtype)
     else:
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
@@ -100,10 +100,10 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     _strided(fields, "gate", gate, x.shape)
     _strided(fields, "x", x, x.shape)
     _strided(fields, "out", out, x.shape)
-    final = dev.empty((sequences, x.shape[-1]), torch.float32, device)
-    states = dev.empty(chunks, torch.float32, device) if return_states else None
+    final = dev.empty(x, (sequences, x.shape[-1]), torch.float32)
+    states = dev.empty(x, chunks, torch.float32) if return_states else None
     args = capi.LinearScanArgs(init=dev.pointer(init), final_state=final.data_ptr(), states=dev.pointer(states), **fields)
-    _run(capi.lib().thrust_cdna4_linear_scan, args, device, "linear_scan")
+    _run(capi.lib().thrust_cdna4_linear_scan, args, device, x, "linear_scan")
     return (out, final, states) if return_states else (out, final)
 
 
@@ -120,14 +120,14 @@ def linear_scan_backward(grad_out, gate, x, states, init=None, grad_final=None, 
         raise ValueError("states must be what linear_scan returned for these shapes")
     if grad_out.dtype != x.dtype:
         raise ValueError("grad_out must have the type of x")
-    grad_gate, grad_x = dev.empty(x.shape, gate.dtype, device), dev.empty(x.shape, x.dtype, device)
-    grad_init = None if init is None else dev.empty(init.shape, torch.float32, device)
+    grad_gate, grad_x = dev.empty(x, x.shape, gate.dtype), dev.empty(x, x.shape, x.dtype)
+    grad_init = None if init is None else dev.empty(x, init.shape, torch.float32)
     fields["clear_outside"] = True
     for name, t in (("gate", gate), ("x", x), ("grad_out", grad_out), ("grad_gate", grad_gate), ("grad_x", grad_x)):
         _strided(fields, name, t, x.shape)
     args = capi.LinearScanBackwardArgs(init=dev.pointer(init), states=states.data_ptr(), grad_final=dev.pointer(grad_final),
                                        grad_init=dev.pointer(grad_init), **fields)
-    _run(capi.lib().thrust_cdna4_linear_scan_backward, args, device, "linear_scan_backward")
+    _run(capi.lib().thrust_cdna4_linear_scan_backward, args, device, x, "linear_scan_backward")
     return grad_gate, grad_x, grad_init
 
 
@@ -139,26 +139,34 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
     device = dev.need_device(gate, x, state, slots, out)
     dev.no_autograd(gate, x, state)
     _types(gate, x)
-    if x.dim() != 2:
+    shape = x.shape
+    if len(shape) != 2:
         raise ValueError("x must be [batch, channels]")
-    batch, channels = x.shape
+    batch, channels = shape
     if state.dim() != 2:
         raise ValueError("state must be [slots, channels]")
-    _state(state, state.shape[0], channels, "state")
+    num_slots = state.shape[0]
+    _state(state, num_slots, channels, "state")
     if slots is None:
-        if batch > state.shape[0]:
+        if batch > num_slots:
             raise ValueError("more rows than slots")
-    elif slots.dtype != torch.int32 or slots.shape != (batch,) or not slots.is_contiguous():
+    elif slots.dtype != torch.int32 or slots.shape != shape[:1] or not slots.is_contiguous():
         raise ValueError("slots must be int32 [batch], contiguous")
     if out is None:
-        out = dev.empty(x.shape, x.dtype, device)
+        out, out_stride = dev.empty(x, shape, x.dtype), channels
     else:
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
-    with dev.current(device):
-        capi.check(capi.lib().thrust_cdna4_linear_scan_step(
-            _DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate.data_ptr(), _rows(gate, x.shape, "gate")[1], x.data_ptr(), _rows(x, x.shape, "x")[1],
-            out.data_ptr(), _rows(out, x.shape, "out")[1], state.data_ptr(), state.shape[0], dev.pointer(slots), batch, channels,
-            dev.stream(device)), "linear_scan_step")
+        out_stride = _rows(out, shape, "out")[1]
+    args = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate.data_ptr(), _rows(gate, shape, "gate")[1], x.data_ptr(), _rows(x, shape, "x")[1],
+            out.data_ptr(), out_stride, state.data_ptr(), num_slots, dev.pointer(slots), batch, channels, dev.stream(device))
+    entry = capi.lib().thrust_cdna4_linear_scan_step
+    if dev.is_current(device):
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
+    if rc:
+        capi.check(rc, "linear_scan_step")
     return out
