@@ -37,6 +37,7 @@ namespace tcd {
 constexpr int kLinWaves = 8;
 constexpr int kLinBlock = kLinWaves * kWave;
 constexpr int kLinGroup = 8;   // tiles of a group, groups of a super-group
+constexpr int kLinTicketWords = 32;
 constexpr int kLinSuper = kLinGroup * kLinGroup;
 constexpr int kLinChunk = THRUST_CDNA4_LINEAR_SCAN_CHUNK;
 constexpr int64_t kLinMaxChannels = int64_t(1) << 28;  // a lane's offset in a row of maps is 32 bits of bytes
@@ -59,7 +60,7 @@ struct LinArgs {
   int64_t rows, channels;
   int sequences, offsets64, log_gate, clear_outside;
   int batch, ntiles, ncb;
-  uint32_t* ticket;
+  uint32_t* tickets;    // [batch][channel blocks], a cache line each
   uint64_t* tile_map;   // [batch][ntiles][channels]
   uint64_t* group_map;  // [batch][groups][channels]
   uint32_t* super_state;  // [batch][super-groups][channels]
@@ -342,20 +343,23 @@ __device__ inline void wave_carry(const LinShared<kWave * VEC>& sm, int lw, int 
   }
 }
 
-// Which tile this workgroup takes: in the order of a ticket where tiles wait for one another (a tile
-// then only waits for running ones), by its index where none does.
+// Which tile this workgroup takes.  Tiles wait for one another along the rows only, so every chain of
+// tiles (a batch's block of channels) has a ticket of its own: a tile then only waits for running ones,
+// and the tickets of a first generation of 512 workgroups, 14 ns each where they all take the same one,
+// are taken side by side.  Without anything to wait for there are no tickets.
 __device__ inline void take_lin_tile(const LinArgs& p, uint32_t* shared, int64_t& i, int& b, int& cb) {
-  uint32_t t = blockIdx.x;
-  if (p.ticket) {
-    if (threadIdx.x == 0) *shared = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    t = (uint32_t)__builtin_amdgcn_readfirstlane((int)*shared);
-  }
   const uint32_t across = (uint32_t)p.batch * (uint32_t)p.ncb;
-  i = t / across;
-  const uint32_t rest = t % across;
-  cb = (int)(rest % (uint32_t)p.ncb);
-  b = (int)(rest / (uint32_t)p.ncb);
+  // each row of workgroups serves every chain once, shifted by one from row to row, so that no chain
+  // stays with one XCD (workgroup k runs on XCD k mod 8) and ends when the slowest of them does
+  const uint32_t chain = (blockIdx.x + blockIdx.x / across) % across;
+  cb = (int)(chain % (uint32_t)p.ncb);
+  b = (int)(chain / (uint32_t)p.ncb);
+  i = blockIdx.x / across;
+  if (p.tickets) {
+    if (threadIdx.x == 0) *shared = atomicAdd(p.tickets + (size_t)chain * kLinTicketWords, 1u);
+    __syncthreads();
+    i = (uint32_t)__builtin_amdgcn_readfirstlane((int)*shared);
+  }
 }
 
 // States of sequences without rows: the final state is the initial one (the gradients likewise).
@@ -807,7 +811,7 @@ inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_row
   l.clear = 0;
   if (l.ntiles > 1) {
     const size_t across = (size_t)batch * (size_t)channels;
-    l.tile_at = 256;
+    l.tile_at = align_up((size_t)batch * (size_t)ncb * kLinTicketWords * 4, 256);
     l.group_at = l.tile_at + align_up(across * (size_t)l.ntiles * 8, 256);
     l.super_at = l.group_at + align_up(across * (size_t)ceil_div(l.ntiles, (int64_t)kLinGroup) * 8, 256);
     l.bytes = l.super_at + align_up(across * (size_t)ceil_div(l.ntiles, (int64_t)kLinSuper) * 4, 256);
@@ -819,10 +823,10 @@ inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_row
 inline void lin_storage(LinArgs& p, const LinPlan& l, void* temp) {
   p.ntiles = (int)l.ntiles;
   p.ncb = l.ncb;
-  p.ticket = nullptr;
+  p.tickets = nullptr;
   if (l.ntiles > 1) {
     char* t = static_cast<char*>(temp);
-    p.ticket = reinterpret_cast<uint32_t*>(t);
+    p.tickets = reinterpret_cast<uint32_t*>(t);
     p.tile_map = reinterpret_cast<uint64_t*>(t + l.tile_at);
     p.group_map = reinterpret_cast<uint64_t*>(t + l.group_at);
     p.super_state = reinterpret_cast<uint32_t*>(t + l.super_at);
