@@ -47,38 +47,40 @@ def _state(t, sequences, channels, what):
         raise ValueError(f"{what} must be float32 [{sequences}, {channels}], contiguous")
 
 
-def _shape(gate, x, offsets, log_gate):
-    """The arguments that say what is computed, the number of sequences and of chunks."""
+def _shape(gate, x, offsets, log_gate, clear_outside):
+    """The arguments that say what is computed, the number of sequences and the shape of the chunks' states."""
     _types(gate, x)
+    shape = x.shape
     if offsets is None:
-        if x.dim() != 3:
+        if len(shape) != 3:
             raise ValueError("x must be [batch, rows, channels], or [rows, channels] with offsets")
-        batch, rows, channels = x.shape
+        batch, rows, channels = shape
         sequences, size = batch, 0
     else:
-        if x.dim() != 2:
+        if len(shape) != 2:
             raise ValueError("x must be [rows, channels] where offsets are given")
         if offsets.dim() != 1 or offsets.dtype not in (torch.int32, torch.int64) or not offsets.is_contiguous() or offsets.numel() < 1:
             raise ValueError("offsets must be int32 or int64 [sequences + 1], contiguous")
-        batch, (rows, channels) = 1, x.shape
+        batch, (rows, channels) = 1, shape
         sequences, size = offsets.numel() - 1, offsets.element_size()
-    fields = dict(gate_dtype=_DT[gate.dtype], x_dtype=_DT[x.dtype], log_gate=bool(log_gate), offset_bytes=size,
-                  batch=batch, rows=rows, channels=channels, sequences=sequences, offsets=dev.pointer(offsets))
+    fields = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), size, clear_outside, batch, rows, channels, sequences)
     return fields, sequences, (batch, -(-rows // capi.LINEAR_SCAN_CHUNK), channels)
 
 
-def _strided(fields, name, t, shape):
-    fields[name] = t.data_ptr()
-    fields[name + "_batch_stride"], fields[name + "_row_stride"] = _rows(t, shape, name)
+def _strided(t, shape, what):
+    return (t.data_ptr(), *_rows(t, shape, what))
 
 
 def _run(entry, args, device, x, what):
+    nbytes, where = ctypes.c_size_t(0), ctypes.byref(args)
+    stream = dev.stream(device)
     with dev.current(device):
-        nbytes = ctypes.c_size_t(0)
-        stream = dev.stream(device)
-        capi.check(entry(None, ctypes.byref(nbytes), ctypes.byref(args), stream), what)
-        temp = dev.empty(x, (nbytes.value,), torch.uint8)
-        capi.check(entry(temp.data_ptr(), ctypes.byref(nbytes), ctypes.byref(args), stream), what)
+        rc = entry(None, ctypes.byref(nbytes), where, stream)
+        if rc == 0:
+            temp = dev.empty(x, (nbytes.value,), torch.uint8)
+            rc = entry(temp.data_ptr(), ctypes.byref(nbytes), where, stream)
+    if rc:
+        capi.check(rc, what)
 
 
 def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, return_states=False):
@@ -88,21 +90,21 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     Packed rows that belong to no sequence are left as they were in a given `out`, and zero in a new one."""
     device = dev.need_device(gate, x, init, offsets, out)
     dev.no_autograd(gate, x, init)
-    fields, sequences, chunks = _shape(gate, x, offsets, log_gate)
-    _state(init, sequences, x.shape[-1], "init")
-    fields["clear_outside"] = out is None
+    fields, sequences, chunks = _shape(gate, x, offsets, log_gate, out is None)
+    shape = x.shape
+    state = (sequences, shape[-1])
+    _state(init, *state, "init")
+    gate_args, x_args = _strided(gate, shape, "gate"), _strided(x, shape, "x")
     if out is None:
-        out = dev.empty(x, x.shape, x.dtype)
+        out = dev.empty(x, shape, x.dtype)
     else:
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
-    _strided(fields, "gate", gate, x.shape)
-    _strided(fields, "x", x, x.shape)
-    _strided(fields, "out", out, x.shape)
-    final = dev.empty(x, (sequences, x.shape[-1]), torch.float32)
+    out_args = _strided(out, shape, "out")
+    final = dev.empty(x, state, torch.float32)
     states = dev.empty(x, chunks, torch.float32) if return_states else None
-    args = capi.LinearScanArgs(init=dev.pointer(init), final_state=final.data_ptr(), states=dev.pointer(states), **fields)
+    args = capi.LinearScanArgs(*fields, *gate_args, *x_args, *out_args, dev.pointer(offsets), dev.pointer(init), final.data_ptr(), dev.pointer(states))
     _run(capi.lib().thrust_cdna4_linear_scan, args, device, x, "linear_scan")
     return (out, final, states) if return_states else (out, final)
 
@@ -113,20 +115,20 @@ def linear_scan_backward(grad_out, gate, x, states, init=None, grad_final=None, 
     `states` are those that linear_scan returned."""
     device = dev.need_device(grad_out, gate, x, states, init, grad_final, offsets)
     dev.no_autograd(grad_out, gate, x, init, grad_final)
-    fields, sequences, chunks = _shape(gate, x, offsets, log_gate)
-    _state(init, sequences, x.shape[-1], "init")
-    _state(grad_final, sequences, x.shape[-1], "grad_final")
+    fields, sequences, chunks = _shape(gate, x, offsets, log_gate, True)
+    shape = x.shape
+    state = (sequences, shape[-1])
+    _state(init, *state, "init")
+    _state(grad_final, *state, "grad_final")
     if states.dtype != torch.float32 or states.shape != chunks or not states.is_contiguous():
         raise ValueError("states must be what linear_scan returned for these shapes")
     if grad_out.dtype != x.dtype:
         raise ValueError("grad_out must have the type of x")
-    grad_gate, grad_x = dev.empty(x, x.shape, gate.dtype), dev.empty(x, x.shape, x.dtype)
-    grad_init = None if init is None else dev.empty(x, init.shape, torch.float32)
-    fields["clear_outside"] = True
-    for name, t in (("gate", gate), ("x", x), ("grad_out", grad_out), ("grad_gate", grad_gate), ("grad_x", grad_x)):
-        _strided(fields, name, t, x.shape)
-    args = capi.LinearScanBackwardArgs(init=dev.pointer(init), states=states.data_ptr(), grad_final=dev.pointer(grad_final),
-                                       grad_init=dev.pointer(grad_init), **fields)
+    inputs = (*_strided(gate, shape, "gate"), *_strided(x, shape, "x"), *_strided(grad_out, shape, "grad_out"))
+    grad_gate, grad_x = dev.empty(x, shape, gate.dtype), dev.empty(x, shape, x.dtype)
+    grad_init = None if init is None else dev.empty(x, state, torch.float32)
+    args = capi.LinearScanBackwardArgs(*fields, *inputs, *_strided(grad_gate, shape, "grad_gate"), *_strided(grad_x, shape, "grad_x"),
+                                       dev.pointer(offsets), dev.pointer(init), states.data_ptr(), dev.pointer(grad_final), dev.pointer(grad_init))
     _run(capi.lib().thrust_cdna4_linear_scan_backward, args, device, x, "linear_scan_backward")
     return grad_gate, grad_x, grad_init
 
