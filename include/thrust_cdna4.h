@@ -188,7 +188,8 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  * columns.  a[t] is gate[t], or exp(gate[t]) when `log_gate` is not 0.
  *
  * Shapes: `batch` sequences of `rows` rows of `channels` elements; element (b, t, c) of an array is
- * at b * batch_stride + t * row_stride + c (strides in elements, not negative; at most 2^28 channels).  Or packed:
+ * at b * batch_stride + t * row_stride + c (strides in elements, not negative).  At most 2^28 channels, and 2^23 workgroups of 64 or 128 rows by
+ * 64 channels (by 128 or 256 from 129 channels on).  Or packed:
  * `offset_bytes` 4 or 8, `offsets` a DEVICE array of sequences + 1 ascending signed integers of that
  * size, batch 1; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none.  Rows
  * in front of the first sequence and behind the last one are part of none: their outputs are left as
@@ -203,7 +204,7 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  * rows, which the gradient needs.  out may be x or gate itself (same address, strides and type); any
  * other overlap of an output with an input is an error that is not detected.
  *
- * Infinities and NaNs stay in their channel and sequence.  Products of factors over up to 512 rows are
+ * Infinities and NaNs stay in their channel and sequence.  Products of factors over up to 1024 rows are
  * formed on their own: where one underflows, an infinite state turns into NaN; where one overflows
  * 32 bits, a state of zero does.  Results are the same from run to run: what
  * is combined with what depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan.
@@ -229,7 +230,7 @@ int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const thrust_cdna4_
  * Its gradient.  From grad_out (the type of x) and `grad_final` (F32, NULL: zero) computes grad_x (the
  * type of x), grad_gate (the type of gate; for log_gate the gradient of the logarithm) and `grad_init`
  * (F32 [sequences or batch][channels], NULL: not wanted; must not overlap init or grad_final), with the
- * recurrence's inputs and the `states` it left.
+ * recurrence's inputs and the `states` it left.  The outputs must not overlap the inputs.
  */
 typedef struct thrust_cdna4_linear_scan_backward_args {
   int gate_dtype, x_dtype, log_gate, offset_bytes, clear_outside;

@@ -36,7 +36,7 @@ def test_size_queries():
 
 @pytest.mark.parametrize("change", [
     dict(gate_dtype=capi.F64), dict(x_dtype=capi.F64, gate_dtype=capi.F64), dict(x_dtype=capi.I32), dict(gate_dtype=capi.F16), dict(x_dtype=99),
-    dict(batch=-1), dict(rows=-1), dict(channels=-1), dict(batch=2 ** 31), dict(channels=2 ** 31), dict(rows=2 ** 50),
+    dict(batch=-1), dict(rows=-1), dict(channels=-1), dict(batch=2 ** 31), dict(channels=2 ** 31), dict(channels=2 ** 28 + 1, rows=1), dict(rows=2 ** 50), dict(batch=1, rows=2 ** 31, channels=256),
     dict(offset_bytes=2, batch=1), dict(offset_bytes=4, batch=2), dict(offset_bytes=8, batch=1, sequences=-1), dict(offset_bytes=8, batch=1, sequences=2 ** 31)],
     ids=str)
 def test_shapes_and_types_refused(change):
@@ -77,7 +77,7 @@ def test_step_refuses():
         return call(gate_dtype, x_dtype, 0, gate, 4, x, 4, out, 4, state, slots_n, slots, batch, channels, None)
     assert rc(batch=0) == 0 and rc(channels=0) == 0
     for bad in (dict(batch=9), dict(batch=-1), dict(channels=-1), dict(slots_n=-1), dict(gate=None), dict(x=None), dict(out=None), dict(state=None),
-                dict(gate_dtype=capi.BF16), dict(x_dtype=capi.F64), dict(batch=2 ** 31, slots_n=2 ** 32), dict(channels=2 ** 31)):
+                dict(gate_dtype=capi.BF16), dict(x_dtype=capi.F64), dict(batch=2 ** 31, slots_n=2 ** 32), dict(channels=2 ** 31), dict(batch=2 ** 24, slots_n=2 ** 24)):
         assert rc(**bad) == INVALID, bad
 
 
@@ -100,7 +100,7 @@ def test_page_calls_refuse():
         assert L.thrust_cdna4_pages_free(ctypes.byref(cache_args(**bad)), 0x5000, 3, None, None) == INVALID, bad
         assert L.thrust_cdna4_pages_compact(t, b, ctypes.byref(cache_args(**bad)), 0x5000, 0x6000, 0x7000, None) == INVALID, bad
     assert calls(cache_args(), temp=0x10004) == {INVALID} and calls(cache_args(), ids=None) == {INVALID} and calls(cache_args(), done=None) == {INVALID}
-    assert calls(cache_args(), n=-1) == {INVALID} and calls(cache_args(), n=(1 << 24) + 1) == {INVALID} and calls(cache_args(), n=0) == {0}
+    assert calls(cache_args(), n=-1) == {INVALID} and calls(cache_args(), n=(1 << 23) + 1) == {INVALID} and calls(cache_args(), n=0) == {0}
     small = ctypes.c_size_t(100)
     assert L.thrust_cdna4_pages_fork(t, ctypes.byref(small), ctypes.byref(cache_args()), 0x5000, 0x5000, 3, 1, 0x6000, None) == INVALID
     assert L.thrust_cdna4_pages_free(None, 0x5000, 3, None, None) == INVALID and L.thrust_cdna4_pages_free(ctypes.byref(cache_args()), 0x5000, 0, None, None) == 0

@@ -9,8 +9,11 @@
 //   c <- a_t g_t,
 // starting from the gradient of the final state and ending in the gradient of the initial one.
 //
-// What bounds it: two additions and two products a value against 6 to 14 bytes of memory; each kernel
-// reads and writes every array once.
+// What bounds it: memory.  Each kernel reads and writes every array once, 6 to 14 bytes a value (a large
+// copy reaches 4.75 TB/s on MI355X).  Measured: 131072 rows of 2048 channels, all 16-bit, 319 us, 5.0 TB/s;
+// 8 x 4096 x 2560 with 32-bit logarithms as gates 149 us, 4.5 TB/s, and its gradient 234 us, 5.0 TB/s.  A
+// short call is bound by the trips to memory one behind the other: 8192 rows of 4096 channels 54 us,
+// 3.7 TB/s.
 //
 // Split.  A workgroup of 8 wavefronts takes a tile of 8 S rows by 64 VEC channels; wavefront w holds S
 // consecutive rows of it in registers, a lane holds VEC neighbouring channels of each.  One pass over
@@ -20,6 +23,13 @@
 // the 64th of a super-group the state itself.  A tile reads at most one state, 7 group maps and 7 tile
 // maps and folds them in the order of the rows: what is combined with what depends on the sizes alone,
 // so results do not vary from run to run.
+//
+// The tile.  S is 16 rows for 16-bit arrays and 8 otherwise: 64 registers of a lane, which leaves two
+// workgroups to a compute unit (128 registers at most).  Half the rows in twice the workgroups took 450 us
+// instead of 408 for the long sequence, twice as many channels in half the rows 816: every halving of
+// the rows doubles the tiles that wait for one another.  80 registers, for three workgroups, spill and
+// took 491.  A first look-back that met in LDS, group maps behind tile maps, took 459 where the present
+// one took 412.
 //
 // Descriptors.  A map is one 64-bit word (A's bits << 32 | H's bits), stored inverted in a single
 // relaxed agent-scope atomic; NaNs are stored as the canonical one, so no map is the word 0, which
@@ -41,7 +51,7 @@ constexpr int kLinTicketWords = 32;
 constexpr int kLinSuper = kLinGroup * kLinGroup;
 constexpr int kLinChunk = THRUST_CDNA4_LINEAR_SCAN_CHUNK;
 constexpr int64_t kLinMaxChannels = int64_t(1) << 28;  // a lane's offset in a row of maps is 32 bits of bytes
-constexpr uint32_t kLinSpinLimit = 1u << 22;
+constexpr uint32_t kLinSpinLimit = 1u << 22;  // polls; seconds
 
 __device__ unsigned int g_linear_scan_timeouts;
 
@@ -226,7 +236,8 @@ __device__ inline float map_shift(uint64_t word) { return bit_cast<float>((uint3
 template <int N, class W>
 __device__ inline void wait_words(const W* p, int64_t stride, uint32_t c, W (&v)[N]) {
   // The ticket order makes every predecessor a running workgroup, so these waits end; the limit keeps a
-  // mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts).
+  // mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts); what was waited for
+  // then reads as NaN.
   for (uint32_t spins = 0;; spins++) {
     bool all = true;
 #pragma unroll
@@ -683,9 +694,11 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
 
 // ---------------------------------------------------------------------------------------
 // One token for each of a batch: state[slot] = a state[slot] + x, out = state.  Rows of one slot are
-// taken in their order: the first of them does all, the others leave.  What bounds it is memory; to
-// know whether a row is the first of its slot a workgroup reads all slots, 16 bytes a thread, which is
-// why it takes UNIT vectors of channels a thread where the batch fills the device all the same.
+// taken in their order: the first of them does all, the others leave.  What bounds it is memory: 2048
+// rows of 8192 16-bit channels take 49 us, 4.8 TB/s.  To know whether a row is the first of its slot a
+// workgroup reads all slots, 16 bytes a thread; with one wavefront reading 4 bytes a lane, and four
+// times as many workgroups, the same batch took 89 us.  So a thread takes UNITS = 4 vectors where that
+// leaves two workgroups to a compute unit, and one in a small batch (8 x 1024: 3.8 us on the device).
 // ---------------------------------------------------------------------------------------
 constexpr int kStepBlock = 256;
 constexpr int kStepWide = 4;  // vectors a thread takes in a large batch
@@ -805,7 +818,7 @@ inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_row
   const int64_t ncb = ceil_div(channels, (int64_t)kWave * l.vec);
   l.ntiles = rows > 0 ? ceil_div(rows, (int64_t)tile_rows) : 1;
   const double grid = (double)ncb * (double)batch * (double)l.ntiles;
-  if (grid > 2147483647.0) return false;
+  if (grid * kLinBlock >= 4294967296.0) return false;  // a launch counts its threads in 32 bits
   l.ncb = (int)ncb;
   l.bytes = 256;
   l.clear = 0;
@@ -849,8 +862,10 @@ inline size_t span_bytes(int64_t batch, int64_t rows, int64_t channels, int64_t 
   return (size_t)((batch - 1) * bs + (rows - 1) * rs + channels) * (size_t)elem;
 }
 
-// Four channels a lane where half of a wavefront's lanes find work, one otherwise.  An output over an
-// input allows the former only where no vector reaches over a workgroup's channels.
+// Four channels a lane where more than half of a wavefront's lanes find work, one otherwise: training
+// pass of 60000 rows, 16-bit, 64 channels 62 us with one and 75 with four, 128 channels 76 and 79, 160
+// channels 97 and 82, 512 channels 209 and 139.  An output over an input allows four only where no
+// vector reaches over a workgroup's channels: the neighbour may have replaced what it repeats.
 inline bool lin_narrow(int64_t channels, bool in_place) { return channels <= 128 || (in_place && channels % 4 != 0); }
 
 }  // namespace tcd
@@ -928,24 +943,13 @@ extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes,
   const bool packed = a->offset_bytes != 0;
   if (!valid_shape(a->batch, a->rows, a->channels, a->sequences, a->offsets, a->offset_bytes)) return hipErrorInvalidValue;
   if (!activation_size(a->gate_dtype) || !activation_size(a->x_dtype)) return hipErrorInvalidValue;
-  const int ex = activation_size(a->x_dtype), eg = activation_size(a->gate_dtype);
-  const size_t in_span[3] = {span_bytes(a->batch, a->rows, a->channels, a->x_batch_stride, a->x_row_stride, ex),
-                             span_bytes(a->batch, a->rows, a->channels, a->gate_batch_stride, a->gate_row_stride, eg),
-                             span_bytes(a->batch, a->rows, a->channels, a->grad_out_batch_stride, a->grad_out_row_stride, ex)};
-  const void* in_at[3] = {a->x, a->gate, a->grad_out};
-  const size_t span_dx = span_bytes(a->batch, a->rows, a->channels, a->grad_x_batch_stride, a->grad_x_row_stride, ex);
-  const size_t span_dg = span_bytes(a->batch, a->rows, a->channels, a->grad_gate_batch_stride, a->grad_gate_row_stride, eg);
-  bool in_place = false;
-  for (int k = 0; k < 3; k++)
-    in_place = in_place || (a->grad_x && ranges_overlap(a->grad_x, span_dx, in_at[k], in_span[k])) ||
-               (a->grad_gate && ranges_overlap(a->grad_gate, span_dg, in_at[k], in_span[k]));
   hipError_t rc = hipErrorInvalidValue;
   dispatch_activation(a->gate_dtype, a->x_dtype, [&](auto tg, auto tx) {
     using TG = decltype(tg);
     using TX = decltype(tx);
     LinPlan l;
     constexpr int kWide = sizeof(TX) == 4 ? 2 : 4;  // the payload of a lane: three arrays of 8 rows
-    if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, lin_narrow(a->channels, in_place) ? 1 : kWide, l)) return;
+    if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, lin_narrow(a->channels, false) ? 1 : kWide, l)) return;
     if (temp == nullptr) {
       *temp_bytes = l.bytes;
       rc = hipSuccess;
@@ -1021,7 +1025,7 @@ extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int lo
     const int64_t wide = ceil_div(vectors, (int64_t)kStepBlock * kStepWide);
     const bool many = batch * wide >= 2 * (int64_t)device_cu_count();
     const int64_t ncb = many ? wide : few;
-    if ((double)ncb * (double)batch > 2147483647.0) return;
+    if ((double)ncb * (double)batch * kStepBlock >= 4294967296.0) return;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)(ncb * batch));
     auto go = [&](auto units, auto log) {
