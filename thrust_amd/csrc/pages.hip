@@ -26,7 +26,7 @@ constexpr int kRequestWaves = kPageBlock / kWave;
 // costs the host about 3 us and the device 2 us, the loops over pages and requests less than that.
 constexpr int kSmallBlock = 1024;
 constexpr int kSmallPages = kSmallBlock * kPagesPerThread;
-constexpr int kSmallRequests = 4 * kSmallBlock / kWave;
+constexpr int kSmallRequests = kWave;
 
 struct PageCache {
   const uint64_t* pools;
@@ -108,9 +108,9 @@ __device__ inline void tally_span(const PageCache& c, const PageTemp& t, int spa
   if (threadIdx.x == 0) t.span_free[span] = total;
 }
 
-// f(q, count, free pages before q) for every page of a span, by the whole workgroup; the free pages up to its end
+// f(q, count, free pages before q) for every page of a span, by the whole workgroup
 template <int BLOCK, class F>
-__device__ inline int64_t sweep_span(const PageCache& c, const PageTemp& t, BlockSum<BLOCK>& sm, int span, int64_t before, F f) {
+__device__ inline void sweep_span(const PageCache& c, const PageTemp& t, BlockSum<BLOCK>& sm, int span, int64_t before, F f) {
   const int64_t begin = (int64_t)span * t.span;
   const int64_t end = begin + t.span < c.num_pages ? begin + t.span : c.num_pages;
   for (int64_t at = begin; at < end; at += BLOCK * kPagesPerThread) {
@@ -131,7 +131,26 @@ __device__ inline int64_t sweep_span(const PageCache& c, const PageTemp& t, Bloc
     }
     before += total;
   }
-  return before;
+}
+
+// f(q, count, free pages before q, free pages) for every page of a small cache
+template <int BLOCK, class F>
+__device__ inline int64_t sweep_once(const PageCache& c, BlockSum<BLOCK>& sm, F f) {
+  int n[kPagesPerThread];
+  const int q0 = (int)threadIdx.x * kPagesPerThread;
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < kPagesPerThread; k++) n[k] = q0 + k < c.num_pages ? c.refs[q0 + k] : 1;
+#pragma unroll
+  for (int k = 0; k < kPagesPerThread; k++) mine += n[k] == 0;
+  int total;
+  int rank = block_exclusive(sm, mine, total);
+#pragma unroll
+  for (int k = 0; k < kPagesPerThread; k++) {
+    if (q0 + k < c.num_pages) f(q0 + k, n[k], rank, total);
+    rank += n[k] == 0;
+  }
+  return total;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -159,7 +178,6 @@ __device__ inline bool named_before(const int32_t* named, int64_t i, int s) {
   }
   return __ballot(found) != 0;
 }
-__device__ inline bool named_anywhere(const int32_t* named, int64_t n, int s) { return named_before(named, n, s); }
 
 enum : int { kFork = 0, kForkShared = 1, kResize = 2 };
 
@@ -171,27 +189,31 @@ struct Requests {
   uint8_t* done;
 };
 
-// Shrinks and frees, a wavefront for a request.  need[i] = 0, or -1 where the request is refused.
-__device__ inline void shrink(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
+__device__ inline bool valid_resize(const PageCache& c, int s, int64_t want) {
+  return s >= 0 && s < c.num_sequences && want >= 0 && want <= (int64_t)c.max_pages * c.page_size;
+}
+// Shrinks and frees, a wavefront for a sequence.
+__device__ inline void shrink_rows(const PageCache& c, int s, int want) {
   const int lane = lane_id();
-  const int s = r.named[i];
-  const int64_t want = r.first ? r.first[i] : 0;
-  bool ok = s >= 0 && s < c.num_sequences && want >= 0 && want <= (int64_t)c.max_pages * c.page_size;
-  if (ok) ok = !named_before(r.named, i, s);
-  if (lane == 0) {
-    if (t.need) t.need[i] = ok ? 0 : -1;
-    else if (r.done) r.done[i] = ok;  // pages_free: nothing is left to do
-  }
-  if (!ok) return;
   const int old = __builtin_amdgcn_readfirstlane(clamped_length(c, s));
   if (want >= old) return;
   int32_t* row = c.tables + (int64_t)s * c.max_pages;
-  for (int j = pages_of(c, (int)want) + lane; j < pages_of(c, old); j += kWave) {
+  for (int j = pages_of(c, want) + lane; j < pages_of(c, old); j += kWave) {
     const int q = row[j];
     if (is_page(c, q)) add_count(c, q, -1);
     row[j] = -1;
   }
-  if (lane == 0) c.lengths[s] = (int)want;
+  if (lane == 0) c.lengths[s] = want;
+}
+// need[i] = 0, or -1 where the request is refused
+__device__ inline void shrink(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
+  const int s = r.named[i], want = r.first ? r.first[i] : 0;
+  const bool ok = valid_resize(c, s, want) && !named_before(r.named, i, s);
+  if (lane_id() == 0) {
+    if (t.need) t.need[i] = ok ? 0 : -1;
+    else if (r.done) r.done[i] = ok;  // pages_free: nothing is left to do
+  }
+  if (ok) shrink_rows(c, s, want);
 }
 __global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, PageTemp t, Requests r) {
   const int64_t i = (int64_t)blockIdx.x * kRequestWaves + threadIdx.x / kWave;
@@ -205,25 +227,20 @@ __device__ inline int page_to_copy(const PageCache& c, int s, int old, int want)
   return is_page(c, q) && c.refs[q] > 1 ? q : -1;
 }
 
-// What a resize wants, a thread for a request.
-__device__ inline void want_resize(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
-  if (t.need[i] < 0) return;
+// What a valid resize wants; sets the page that it copies.
+__device__ inline int wanted_by_resize(const PageCache& c, const Requests& r, int64_t i, int32_t& copied) {
   const int s = r.named[i], old = clamped_length(c, s), want = r.first[i];
-  const int q = page_to_copy(c, s, old, want);
-  t.copied[i] = q;
-  t.need[i] = want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (q >= 0);
+  copied = page_to_copy(c, s, old, want);
+  return want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (copied >= 0);
 }
-// What a fork wants, a wavefront for a request.
-__device__ inline void want_fork(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
-  const int parent = r.first[i], child = r.named[i];
-  bool ok = parent >= 0 && parent < c.num_sequences && child >= 0 && child < c.num_sequences;
-  if (ok) ok = c.lengths[child] == 0 && !named_before(r.named, i, child) && !named_anywhere(r.first, r.n, child);
-  int need = -1;
-  if (ok) {
-    const int n = clamped_length(c, parent);
-    need = r.kind == kForkShared ? (n % c.page_size != 0) : pages_of(c, n);
-  }
-  if (lane_id() == 0) t.need[i] = need;
+// What a fork wants that names its child first and no parent as child; -1: refused.
+__device__ inline int wanted_by_fork(const PageCache& c, int kind, int parent, int child) {
+  if (c.lengths[child] != 0) return -1;
+  const int n = clamped_length(c, parent);
+  return kind == kForkShared ? (n % c.page_size != 0) : pages_of(c, n);
+}
+__device__ inline bool valid_fork(const PageCache& c, int parent, int child) {
+  return parent >= 0 && parent < c.num_sequences && child >= 0 && child < c.num_sequences;
 }
 
 // Tallies the free pages and what each request wants.
@@ -232,10 +249,13 @@ __global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, Pa
   const int64_t block = blockIdx.x - t.spans;
   if (r.kind == kResize) {
     const int64_t i = block * kPageBlock + threadIdx.x;
-    if (i < r.n) want_resize(c, t, r, i);
+    if (i < r.n && t.need[i] >= 0) t.need[i] = wanted_by_resize(c, r, i, t.copied[i]);
   } else {
-    const int64_t i = block * kRequestWaves + threadIdx.x / kWave;
-    if (i < r.n) want_fork(c, t, r, i);
+    const int64_t i = block * kRequestWaves + threadIdx.x / kWave;  // a wavefront for a request
+    if (i >= r.n) return;
+    const int parent = r.first[i], child = r.named[i];
+    const bool ok = valid_fork(c, parent, child) && !named_before(r.named, i, child) && !named_before(r.first, r.n, child);
+    if (lane_id() == 0) t.need[i] = ok ? wanted_by_fork(c, r.kind, parent, child) : -1;
   }
 }
 
@@ -264,26 +284,44 @@ __global__ __launch_bounds__(kPageBlock) void pages_list_kernel(PageCache c, Pag
   });
 }
 
-// All of that for a small cache and few requests, in one workgroup instead of two or three launches.
+// All of that for a small cache and up to 64 requests, in one workgroup instead of two or three
+// launches.  The first wavefront has a request in each lane and compares them in registers.
 __global__ __launch_bounds__(kSmallBlock) void pages_plan_small_kernel(PageCache c, PageTemp t, Requests r) {
   __shared__ BlockSum<kSmallBlock> sm;
-  const int w = threadIdx.x / kWave, i = threadIdx.x;
+  __shared__ int s_need[kWave];
+  const int w = threadIdx.x / kWave, i = threadIdx.x, n = (int)r.n;
+  if (w == 0) {
+    const int first = r.first[i < n ? i : 0], named = r.named[i < n ? i : 0];
+    bool again = false, parent = false;
+    for (int j = 0; j < n; j++) {
+      const int child_j = __builtin_amdgcn_readlane(named, j), first_j = __builtin_amdgcn_readlane(first, j);
+      again = again || (j < i && child_j == named);
+      parent = parent || first_j == named;
+    }
+    int need = -1;
+    if (i < n && !again) {
+      if (r.kind == kResize) need = valid_resize(c, named, first) ? 0 : -1;
+      else if (!parent && valid_fork(c, first, named)) need = wanted_by_fork(c, r.kind, first, named);
+    }
+    s_need[i] = need;
+  }
+  __syncthreads();
   if (r.kind == kResize) {
-    for (int64_t k = w; k < r.n; k += kSmallBlock / kWave) shrink(c, t, r, k);
-    __threadfence();  // lengths, counts and needs are read by other wavefronts below
-    __syncthreads();
-    if (i < r.n) want_resize(c, t, r, i);
-  } else {
-    for (int64_t k = w; k < r.n; k += kSmallBlock / kWave) want_fork(c, t, r, k);
-    __threadfence();
+    for (int k = w; k < n; k += kSmallBlock / kWave)
+      if (s_need[k] == 0) shrink_rows(c, r.named[k], r.first[k]);
+    __threadfence();  // lengths, tables and counts are read by other wavefronts below
     __syncthreads();
   }
-  const int64_t need = i < r.n && t.need[i] > 0 ? t.need[i] : 0;
+  int need = i < n ? s_need[i] : 0;
+  if (i < n) {
+    if (r.kind == kResize && need == 0) need = wanted_by_resize(c, r, i, t.copied[i]);
+    t.need[i] = need;
+  }
   int64_t wanted;
-  const int64_t start = block_exclusive(sm, need, wanted);
-  if (i < r.n) t.start[i] = start;
-  const int64_t free = sweep_span(c, t, sm, 0, 0, [&](int64_t q, int count, int64_t rank) {
-    if (count == 0 && rank < wanted) t.free_list[rank] = (int)q;
+  const int64_t start = block_exclusive(sm, (int64_t)(need > 0 ? need : 0), wanted);
+  if (i < n) t.start[i] = start;
+  const int64_t free = sweep_once(c, sm, [&](int q, int count, int rank, int) {
+    if (count == 0 && rank < wanted) t.free_list[rank] = q;
   });
   if (i == 0) t.head[1] = free;
 }
@@ -392,43 +430,38 @@ __global__ __launch_bounds__(kPageBlock) void pages_serve_kernel(PageCache c, Pa
 // ---------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kPageBlock) void pages_tally_only_kernel(PageCache c, PageTemp t) { tally_span(c, t, (int)blockIdx.x); }
 
-template <int BLOCK>
-__device__ inline void rank_span(const PageCache& c, const PageTemp& t, BlockSum<BLOCK>& sm, int span, int64_t before, int64_t live, int32_t* refs_out,
-                                 int32_t* live_out) {
-  if (span == 0 && threadIdx.x == 0) {
-    *live_out = (int)live;
-    if (live == c.num_pages) t.head[0] = 0;
-  }
-  sweep_span(c, t, sm, span, before, [&](int64_t q, int count, int64_t rank) {
-    if (q == live) t.head[0] = rank;  // holes below
-    if (q < live) {
-      if (count == 0) t.free_list[rank] = (int)q;
-      else refs_out[q] = count;
-    } else {
-      int k = -1;
-      if (count != 0) {
-        k = (int)(live - 1 - (q - rank));
-        t.movers[k] = (int)q;
-        t.mover_refs[k] = count;
-      }
-      t.place[q] = k;
-      refs_out[q] = 0;
+__device__ inline void rank_page(const PageTemp& t, int64_t q, int count, int64_t rank, int64_t live, int32_t* refs_out) {
+  if (q == live) t.head[0] = rank;  // holes below
+  if (q < live) {
+    if (count == 0) t.free_list[rank] = (int)q;
+    else refs_out[q] = count;
+  } else {
+    int k = -1;
+    if (count != 0) {
+      k = (int)(live - 1 - (q - rank));
+      t.movers[k] = (int)q;
+      t.mover_refs[k] = count;
     }
-  });
+    t.place[q] = k;
+    refs_out[q] = 0;
+  }
+}
+__device__ inline void publish_live(const PageCache& c, const PageTemp& t, int64_t live, int32_t* live_out) {
+  *live_out = (int)live;
+  if (live == c.num_pages) t.head[0] = 0;  // no page is the first one behind
 }
 __global__ __launch_bounds__(kPageBlock) void pages_rank_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
   __shared__ BlockSum<kPageBlock> sm;
   const int64_t before = block_sum(sm, t.span_free, blockIdx.x);
   const int64_t live = c.num_pages - block_sum(sm, t.span_free, t.spans);
-  rank_span(c, t, sm, (int)blockIdx.x, before, live, refs_out, live_out);
+  if (blockIdx.x == 0 && threadIdx.x == 0) publish_live(c, t, live, live_out);
+  sweep_span(c, t, sm, (int)blockIdx.x, before, [&](int64_t q, int count, int64_t rank) { rank_page(t, q, count, rank, live, refs_out); });
 }
 // The same for a small cache, in one workgroup that needs no tally of spans.
 __global__ __launch_bounds__(kSmallBlock) void pages_rank_small_kernel(PageCache c, PageTemp t, int32_t* refs_out, int32_t* live_out) {
   __shared__ BlockSum<kSmallBlock> sm;
-  int used = 0, live;
-  for (int q = threadIdx.x; q < c.num_pages; q += kSmallBlock) used += c.refs[q] != 0;
-  block_exclusive(sm, used, live);
-  rank_span(c, t, sm, 0, 0, live, refs_out, live_out);
+  const int64_t free = sweep_once(c, sm, [&](int q, int count, int rank, int total) { rank_page(t, q, count, rank, c.num_pages - total, refs_out); });
+  if (threadIdx.x == 0) publish_live(c, t, c.num_pages - free, live_out);
 }
 
 __global__ __launch_bounds__(kPageBlock) void pages_move_kernel(PageCache c, PageTemp t, int32_t* tables_out, int32_t* refs_out,
@@ -509,16 +542,8 @@ static hipError_t grant(const PageCache& c, const PageTemp& t, const Requests& r
   return hipGetLastError();
 }
 
-// one span for a small cache
-static bool small_cache(const PageCache& c, PageTemp& t) {
-  if (c.num_pages > kSmallPages) return false;
-  t.span = kSmallPages;
-  t.spans = 1;
-  return true;
-}
-
-static hipError_t serve(const PageCache& c, PageTemp t, const Requests& r, hipStream_t s) {
-  if (r.n <= kSmallRequests && small_cache(c, t)) {
+static hipError_t serve(const PageCache& c, const PageTemp& t, const Requests& r, hipStream_t s) {
+  if (r.n <= kSmallRequests && c.num_pages <= kSmallPages) {
     TCD_LAUNCH("pages_plan_small_kernel", pages_plan_small_kernel, dim3(1), dim3(kSmallBlock), s, c, t, r);
     return grant(c, t, r, s);
   }
@@ -598,7 +623,7 @@ extern "C" int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const 
     if (e != hipSuccess) return (int)e;
     e = zero_async(t.head, 16, s);
     if (e != hipSuccess) return (int)e;
-  } else if (small_cache(c, t)) {
+  } else if (c.num_pages <= kSmallPages) {
     TCD_LAUNCH("pages_rank_small_kernel", pages_rank_small_kernel, dim3(1), dim3(kSmallBlock), s, c, t, refs_out, live_out);
   } else {
     TCD_LAUNCH("pages_tally_only_kernel", pages_tally_only_kernel, dim3((unsigned)t.spans), dim3(kPageBlock), s, c, t);
