@@ -263,6 +263,37 @@ def test_gradient_against_differences():
     assert abs(got - difference) <= own + 2 * e * e / 6 * third + 2.0 ** -53 / e * 1e3
 
 
+class Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, x, init):
+        out, final, states = thrust_amd.linear_scan(gate, x, init=init, return_states=True)
+        ctx.save_for_backward(gate, x, init, states)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_final):
+        gate, x, init, states = ctx.saved_tensors
+        return thrust_amd.linear_scan_backward(grad_out.contiguous(), gate, x, states, init=init, grad_final=grad_final.contiguous())
+
+
+def test_as_a_function_of_torch():
+    """A model's layer: the two halves of a projection go in, a loss that sums comes back expanded."""
+    gate, x, init, _, _ = inputs(19, (2, 90, 6), 2, F32, F32, True)
+    leaf, h0 = put(torch.cat([gate, x], -1)).requires_grad_(), put(init).requires_grad_()
+    with pytest.raises(ValueError):
+        thrust_amd.linear_scan(*leaf.chunk(2, -1), init=h0)
+    g, v = leaf.chunk(2, -1)
+    out, final = Scan.apply(g.exp(), v, h0)
+    (out.sum() + 3 * final.sum()).backward()
+    ref = Recurrence(gate, x, init, None, True).gradient(torch.ones_like(x), torch.full_like(init, 3))
+    # torch's exp and its gradient add at most two units in the last place to a gate's factor and one product: covered twice over by the
+    # bound for logarithms, whose own exp is counted in it
+    check(get(leaf.grad)[..., :6], ref.grad_gate, 2 * ref.error_gate, "gate")
+    check(get(leaf.grad)[..., 6:], ref.grad_x, 2 * ref.error_x, "x")
+    check(get(h0.grad), ref.grad_init, 2 * ref.error_init, "init")
+
+
 # ---------------------------------------------------------------------------------------
 # The step
 # ---------------------------------------------------------------------------------------

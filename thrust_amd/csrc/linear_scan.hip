@@ -734,6 +734,8 @@ __global__ __launch_bounds__(kStepBlock) void linear_scan_step_kernel(const TG* 
     for (int u = 0; u < UNITS; u++) store(out + (int64_t)row * out_rs, u, Pack<TX, VEC>{});
     return;
   }
+  // Asked for before it is known that the row is the first of its slot: one that is not may read the state
+  // while the first replaces it, and leaves without using what it read.
   float* own = state + (int64_t)slot * C;
   Pack<TG, VEC> g[UNITS];
   Pack<TX, VEC> v[UNITS];
