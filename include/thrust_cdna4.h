@@ -188,12 +188,12 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  * columns.  a[t] is gate[t], or exp(gate[t]) when `log_gate` is not 0.
  *
  * Shapes: `batch` sequences of `rows` rows of `channels` elements; element (b, t, c) of an array is
- * at b * batch_stride + t * row_stride + c (strides in elements, not negative).  At most 2^28 channels, and 2^23 workgroups of 64 or 128 rows by
- * 64 channels (by 128 or 256 from 129 channels on).  Or packed:
- * `offset_bytes` 4 or 8, `offsets` a DEVICE array of sequences + 1 ascending signed integers of that
- * size, batch 1; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none.  Rows
- * in front of the first sequence and behind the last one are part of none: their outputs are left as
- * they were, or zero if `clear_outside` is not 0.  Offsets that do not ascend or that leave the rows
+ * at b * batch_stride + t * row_stride + c (strides in elements, not negative).  At most 2^28
+ * channels, and 2^23 workgroups of 64 or 128 rows by 64 channels (by 128 or 256 from 129 channels on).
+ * Or packed: `offset_bytes` 4 or 8, `offsets` a DEVICE array of sequences + 1 ascending signed integers
+ * of that size, batch 1; sequence s is the rows offsets[s] .. offsets[s + 1] - 1, which may be none.
+ * Rows in front of the first sequence and behind the last one are part of none: their outputs are left
+ * as they were, or zero if `clear_outside` is not 0.  Offsets that do not ascend or that leave the rows
  * give unspecified values, but no access outside the arrays.
  *
  * Types: x and out are F32, F16 or BF16; the gates are of the same type or F32.  Arithmetic and
@@ -206,8 +206,9 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  *
  * Infinities and NaNs stay in their channel and sequence.  Products of factors over up to 1024 rows are
  * formed on their own: where one underflows, an infinite state turns into NaN; where one overflows
- * 32 bits, a state of zero does.  Results are the same from run to run: what
- * is combined with what depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan.
+ * 32 bits, a state of zero does.  Results are the same from run to run: what is combined with what
+ * depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan; up to
+ * THRUST_CDNA4_LINEAR_SCAN_CHUNK rows need none, and then only a non-null address and a size of 256.
  */
 #define THRUST_CDNA4_LINEAR_SCAN_CHUNK 64
 typedef struct thrust_cdna4_linear_scan_args {

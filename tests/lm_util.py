@@ -25,6 +25,7 @@ if EMULATED:
         return api.torch.empty(shape, torch.int16 if two else dtype).view(dtype)
 
     device.need_device = _cpu
+    device.empty_like = lambda t: _empty(t, t.shape, t.dtype)
     device.current = lambda d: contextlib.nullcontext()
     device.is_current = lambda d: True
     device.stream = lambda d: ctypes.c_void_p(0)

@@ -99,6 +99,7 @@ PACKED = {
     "single rows": ([1] * 300, 0, 300),
     "many, ragged": ([(i * 37) % 23 for i in range(200)], 5, 2300),
     "two long ones that meet inside a tile": ([700, 900], 0, 1600),
+    "hundreds of empty ones in one place": ([3] + [0] * 200 + [1, 40] + [0] * 64 + [30] + [0] * 70, 0, 80),
 }
 
 
@@ -337,6 +338,19 @@ def test_step_padding_and_rows_of_one_slot():
     check(out, want, error, "out")
     check(get(on), after, error_state, "state")
     assert (out[(slots < 0) | (slots >= 20)] == 0).all()
+
+
+def test_step_of_a_large_batch_with_rows_of_one_slot():
+    gate, x, _, _, _ = inputs(32, (2500, 5), 2500, F32, F32, False)
+    g = torch.Generator().manual_seed(6)
+    state = torch.randn((3000, 5), generator=g)
+    slots = torch.randperm(3000, generator=g)[:2500].int()
+    slots[2400], slots[7], slots[1300], slots[1301], slots[2499] = slots[3], slots[1027], slots[1299], slots[1299], -1
+    on = put(state)
+    out = thrust_amd.linear_scan_step(put(gate), put(x), on, slots=put(slots))
+    want, after, error, error_state = step_reference(gate, x, state, slots.tolist(), False)
+    check(get(out), want, error, "out")
+    check(get(on), after, error_state, "state")
 
 
 def test_step_is_a_scan_of_one_row_and_takes_halves_of_a_projection():

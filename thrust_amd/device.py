@@ -41,6 +41,11 @@ def empty(like, shape, dtype):
     return like.new_empty(shape, dtype=dtype)
 
 
+def empty_like(t):
+    """Uninitialised and contiguous, of the shape and type of `t`, which costs less to say than a shape."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def pointer(t):
     return None if t is None else t.data_ptr()
 

@@ -28,21 +28,21 @@ class PageCache:
         if not pools:
             raise ValueError("a cache needs a pool")
         device = dev.need_device(*pools, tables, lengths, refs)
+        pages = pools[0].shape[0] if pools[0].dim() else -1
+        total = pools[0].numel() * pools[0].element_size()
         for p in pools:
-            if p.dim() < 1 or not p.is_contiguous() or p.shape[0] != pools[0].shape[0]:
+            if p.dim() < 1 or p.shape[0] != pages or not p.is_contiguous():
                 raise ValueError("pools must be contiguous and of the same number of pages")
-        page_bytes = {p[0].numel() * p.element_size() for p in pools} if pools[0].shape[0] else {0}
-        if len(page_bytes) > 1:
-            raise ValueError("pools must have the same number of bytes a page")
+            if p.numel() * p.element_size() != total:
+                raise ValueError("pools must have the same number of bytes a page")
         if page_size < 1 or max_sequences < 0 or max_pages < 0 or page_size * max_pages > 0x7fffffff:
             raise ValueError("page_size must be positive, and page_size * max_pages below 2^31")
-        pages = pools[0].shape[0]
         self.pools, self.page_size, self.device = pools, page_size, device
         self.tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
         self.lengths = self._array(lengths, (max_sequences,), 0, "lengths")
         self.refs = self._array(refs, (pages,), 0, "refs")
         self._pointers = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device)
-        self._args = capi.PageCacheArgs(pools=self._pointers.data_ptr(), page_bytes=page_bytes.pop(), num_pools=len(pools), num_pages=pages,
+        self._args = capi.PageCacheArgs(pools=self._pointers.data_ptr(), page_bytes=total // max(pages, 1), num_pools=len(pools), num_pages=pages,
                                         page_size=page_size, num_sequences=max_sequences, max_pages=max_pages,
                                         tables=self.tables.data_ptr(), lengths=self.lengths.data_ptr(), refs=self.refs.data_ptr())
         self._ref = ctypes.byref(self._args)

@@ -71,12 +71,17 @@ def _strided(t, shape, what):
     return (t.data_ptr(), *_rows(t, shape, what))
 
 
-def _run(entry, args, device, x, what):
+_ONE_TILE = ctypes.c_size_t(256)
+_UNUSED = 256  # an address that is never used
+
+
+def _run(entry, args, rows, device, x, what):
     nbytes, where = ctypes.c_size_t(0), ctypes.byref(args)
     stream = dev.stream(device)
     with dev.current(device):
-        rc = entry(None, ctypes.byref(nbytes), where, stream)
-        if rc == 0:
+        if rows <= capi.LINEAR_SCAN_CHUNK:  # a single tile has nothing to store: no query, no allocation
+            rc = entry(_UNUSED, ctypes.byref(_ONE_TILE), where, stream)
+        elif (rc := entry(None, ctypes.byref(nbytes), where, stream)) == 0:
             temp = dev.empty(x, (nbytes.value,), torch.uint8)
             rc = entry(temp.data_ptr(), ctypes.byref(nbytes), where, stream)
     if rc:
@@ -96,16 +101,16 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     _state(init, *state, "init")
     gate_args, x_args = _strided(gate, shape, "gate"), _strided(x, shape, "x")
     if out is None:
-        out = dev.empty(x, shape, x.dtype)
+        out = dev.empty_like(x)
     else:
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
     out_args = _strided(out, shape, "out")
-    final = dev.empty(x, state, torch.float32)
+    final = dev.empty(x, state, torch.float32) if init is None else dev.empty_like(init)
     states = dev.empty(x, chunks, torch.float32) if return_states else None
     args = capi.LinearScanArgs(*fields, *gate_args, *x_args, *out_args, dev.pointer(offsets), dev.pointer(init), final.data_ptr(), dev.pointer(states))
-    _run(capi.lib().thrust_cdna4_linear_scan, args, device, x, "linear_scan")
+    _run(capi.lib().thrust_cdna4_linear_scan, args, shape[-2], device, x, "linear_scan")
     return (out, final, states) if return_states else (out, final)
 
 
@@ -125,11 +130,11 @@ def linear_scan_backward(grad_out, gate, x, states, init=None, grad_final=None, 
     if grad_out.dtype != x.dtype:
         raise ValueError("grad_out must have the type of x")
     inputs = (*_strided(gate, shape, "gate"), *_strided(x, shape, "x"), *_strided(grad_out, shape, "grad_out"))
-    grad_gate, grad_x = dev.empty(x, shape, gate.dtype), dev.empty(x, shape, x.dtype)
-    grad_init = None if init is None else dev.empty(x, state, torch.float32)
+    grad_gate, grad_x = dev.empty_like(gate), dev.empty_like(x)
+    grad_init = None if init is None else dev.empty_like(init)
     args = capi.LinearScanBackwardArgs(*fields, *inputs, *_strided(grad_gate, shape, "grad_gate"), *_strided(grad_x, shape, "grad_x"),
                                        dev.pointer(offsets), dev.pointer(init), states.data_ptr(), dev.pointer(grad_final), dev.pointer(grad_init))
-    _run(capi.lib().thrust_cdna4_linear_scan_backward, args, device, x, "linear_scan_backward")
+    _run(capi.lib().thrust_cdna4_linear_scan_backward, args, shape[-2], device, x, "linear_scan_backward")
     return grad_gate, grad_x, grad_init
 
 
@@ -155,7 +160,7 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
     elif slots.dtype != torch.int32 or slots.shape != shape[:1] or not slots.is_contiguous():
         raise ValueError("slots must be int32 [batch], contiguous")
     if out is None:
-        out, out_stride = dev.empty(x, shape, x.dtype), channels
+        out, out_stride = dev.empty_like(x), channels
     else:
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
