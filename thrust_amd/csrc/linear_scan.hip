@@ -10,8 +10,8 @@
 // starting from the gradient of the final state and ending in the gradient of the initial one.
 //
 // What bounds it: memory.  Each kernel reads and writes every array once, 6 to 14 bytes a value (a large
-// copy reaches 4.75 TB/s on MI355X).  Measured: 131072 rows of 2048 channels, all 16-bit, 319 us, 5.0 TB/s;
-// 8 x 4096 x 2560 with 32-bit logarithms as gates 149 us, 4.5 TB/s, and its gradient 234 us, 5.0 TB/s.  A
+// copy reaches 4.75 TB/s on MI355X).  Measured: 131072 rows of 2048 channels, all 16-bit, 307 us, 5.3 TB/s;
+// 8 x 4096 x 2560 with 32-bit logarithms as gates 153 us, 4.4 TB/s, and its gradient 235 us, 5.0 TB/s.  A
 // short call is bound by the trips to memory one behind the other: 8192 rows of 4096 channels 54 us,
 // 3.7 TB/s.
 //
@@ -38,8 +38,6 @@
 // Sequences.  A row that begins a sequence takes its initial state by selection, never by a product
 // with zero, so infinities and NaNs of one sequence stay in it.  Which predecessors a tile needs
 // follows from the offsets alone, as does whether a published map begins anew.
-#include <atomic>
-
 #include "lm_types.h"
 
 namespace tcd {
@@ -695,10 +693,10 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
 // ---------------------------------------------------------------------------------------
 // One token for each of a batch: state[slot] = a state[slot] + x, out = state.  Rows of one slot are
 // taken in their order: the first of them does all, the others leave.  What bounds it is memory: 2048
-// rows of 8192 16-bit channels take 49 us, 4.8 TB/s.  To know whether a row is the first of its slot a
+// rows of 8192 16-bit channels take 47 us, 5.0 TB/s.  To know whether a row is the first of its slot a
 // workgroup reads all slots, 16 bytes a thread; with one wavefront reading 4 bytes a lane, and four
 // times as many workgroups, the same batch took 89 us.  So a thread takes UNITS = 4 vectors where that
-// leaves two workgroups to a compute unit, and one in a small batch (8 x 1024: 3.8 us on the device).
+// leaves two workgroups to a compute unit, and one in a small batch (8 x 1024: 3.5 us on the device).
 // ---------------------------------------------------------------------------------------
 constexpr int kStepBlock = 256;
 constexpr int kStepWide = 4;  // vectors a thread takes in a large batch

@@ -8,9 +8,10 @@
 //
 // What bounds it: with data to move, memory, each byte read and written once (500 forks of 48 pools,
 // 786 MB: 155 us of copying, 5.1 TB/s, and 14 us of the launches before it; 16 KiB a workgroup at a time,
-// four 16-byte loads of a thread in flight).  Without, the launches: 1500 requests on 2^20 pages 30 us in
-// five, of which the counts' 4 MB are 7; a cache of up to 8192 pages with up to 64 requests is planned by
-// one workgroup in one launch (9 requests on 300 pages: 24 us a tick in five launches, 17 in three).
+// four 16-byte loads of a thread in flight).  Without, the launches: 1500 sequences freed and replaced on
+// 2^20 pages 28.6 us in five, of which listing 4 MB of counts is 6; a cache of up to 8192 pages with up to
+// 64 requests is planned by one workgroup in one launch (9 sequences replaced on 300 pages: 24 us in five
+// launches, 16 in three).
 #include "lm_types.h"
 
 namespace tcd {
@@ -88,8 +89,15 @@ __device__ inline T block_exclusive(BlockSum<BLOCK>& sm, T v, T& total) {
 // the sum of the positive ones of n values, the same in all threads
 template <int BLOCK>
 __device__ inline int64_t block_sum(BlockSum<BLOCK>& sm, const int32_t* v, int64_t n) {
+  constexpr int N = 8;  // values of a thread in flight
   int64_t mine = 0, total;
-  for (int64_t i = threadIdx.x; i < n; i += BLOCK) mine += v[i] > 0 ? v[i] : 0;
+  for (int64_t i = threadIdx.x; i < n; i += N * BLOCK) {
+    int u[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) u[k] = v[i + k * BLOCK < n ? i + k * BLOCK : i];
+#pragma unroll
+    for (int k = 0; k < N; k++) mine += i + k * BLOCK < n && u[k] > 0 ? u[k] : 0;
+  }
   block_exclusive(sm, mine, total);
   return total;
 }
@@ -160,21 +168,20 @@ __device__ inline int64_t sweep_once(const PageCache& c, BlockSum<BLOCK>& sm, F 
 // 16 bytes a lane and four of them in flight, 1024 requests a trip
 __device__ inline bool named_before(const int32_t* named, int64_t i, int s) {
   bool found = false;
-  int64_t q0 = (int64_t)lane_id() * 4;
-  for (; q0 + 3 * 4 * kWave + 4 <= i; q0 += 4 * 4 * kWave) {
-    tcd_v4u v[4];
+  if (i < 4) {
+    if (lane_id() < i) found = named[lane_id()] == s;
+  } else {
+    for (int64_t q0 = (int64_t)lane_id() * 4; q0 < i; q0 += 4 * 4 * kWave) {
+      tcd_v4u v[4];  // behind the end, the last four again
 #pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = *reinterpret_cast<const tcd_v4u_anywhere*>(named + q0 + k * 4 * kWave);
+      for (int k = 0; k < 4; k++) {
+        const int64_t q = q0 + k * 4 * kWave;
+        v[k] = *reinterpret_cast<const tcd_v4u_anywhere*>(named + (q + 4 <= i ? q : i - 4));
+      }
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      found = found || (int)v[k][0] == s || (int)v[k][1] == s || (int)v[k][2] == s || (int)v[k][3] == s;
-  }
-  for (; q0 < i; q0 += 4 * kWave) {
-    int v[4];  // behind the end, the last one again, which is an earlier one too
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = named[q0 + k < i ? q0 + k : i - 1];
-#pragma unroll
-    for (int k = 0; k < 4; k++) found = found || v[k] == s;
+      for (int k = 0; k < 4; k++)
+        found = found || (int)v[k][0] == s || (int)v[k][1] == s || (int)v[k][2] == s || (int)v[k][3] == s;
+    }
   }
   return __ballot(found) != 0;
 }
@@ -198,10 +205,19 @@ __device__ inline void shrink_rows(const PageCache& c, int s, int want) {
   const int old = __builtin_amdgcn_readfirstlane(clamped_length(c, s));
   if (want >= old) return;
   int32_t* row = c.tables + (int64_t)s * c.max_pages;
-  for (int j = pages_of(c, want) + lane; j < pages_of(c, old); j += kWave) {
-    const int q = row[j];
-    if (is_page(c, q)) add_count(c, q, -1);
-    row[j] = -1;
+  constexpr int N = 4;  // entries of a lane in flight
+  const int end = pages_of(c, old);
+  for (int j0 = pages_of(c, want) + lane; j0 < end; j0 += N * kWave) {
+    int q[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) q[k] = row[j0 + k * kWave < end ? j0 + k * kWave : j0];
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if (j0 + k * kWave < end) {
+        if (is_page(c, q[k])) add_count(c, q[k], -1);
+        row[j0 + k * kWave] = -1;
+      }
+    }
   }
   if (lane == 0) c.lengths[s] = want;
 }
@@ -263,13 +279,22 @@ __global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, Pa
 __global__ __launch_bounds__(kPageBlock) void pages_list_kernel(PageCache c, PageTemp t, int64_t n) {
   __shared__ BlockSum<kPageBlock> sm;
   if ((int)blockIdx.x == t.spans) {
+    constexpr int N = 8;  // requests of a thread, next to one another
     int64_t sum = 0;
-    for (int64_t at = 0; at < n; at += kPageBlock) {
-      const int64_t i = at + threadIdx.x;
-      const int64_t need = i < n && t.need[i] > 0 ? t.need[i] : 0;
-      int64_t total;
-      const int64_t before = block_exclusive(sm, need, total);
-      if (i < n) t.start[i] = sum + before;
+    for (int64_t at = 0; at < n; at += N * kPageBlock) {
+      const int64_t i0 = at + (int64_t)threadIdx.x * N;
+      int need[N];
+      int64_t mine = 0, total;
+#pragma unroll
+      for (int k = 0; k < N; k++) need[k] = t.need[i0 + k < n ? i0 + k : n - 1];
+#pragma unroll
+      for (int k = 0; k < N; k++) mine += need[k] = i0 + k < n && need[k] > 0 ? need[k] : 0;
+      int64_t start = sum + block_exclusive(sm, mine, total);
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        if (i0 + k < n) t.start[i0 + k] = start;
+        start += need[k];
+      }
       sum += total;
     }
     const int64_t free = block_sum(sm, t.span_free, t.spans);
