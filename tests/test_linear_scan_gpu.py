@@ -144,6 +144,38 @@ def test_halves_of_a_projection_and_outputs_in_place(channels):
     check(get(got), ref1.out, ref1.error_out, "expanded")
 
 
+@pytest.mark.parametrize("channels", [3, 133, 260])
+def test_gradient_of_halves_and_of_interleaved_batches(channels):
+    shape = (2, 150, channels)
+    gate, x, init, grad_out, grad_final = inputs(21, shape, 2, F16, F16, False)
+    ref = Recurrence(gate, x, init, None, False).gradient(grad_out, grad_final)
+    both = put(torch.cat([gate, x], -1))
+    g, v = both[..., :channels], both[..., channels:]
+    d = put(grad_out.transpose(0, 1).contiguous()).transpose(0, 1)
+    states = thrust_amd.linear_scan(g, v, init=put(init), return_states=True)[2]
+    grads = thrust_amd.linear_scan_backward(d, g, v, states, init=put(init), grad_final=put(grad_final))
+    assert all(t.is_contiguous() for t in grads)
+    check(get(grads[0]), ref.grad_gate, ref.error_gate, "grad_gate")
+    check(get(grads[1]), ref.grad_x, ref.error_x, "grad_x")
+    check(get(grads[2]), ref.grad_init, ref.error_init, "grad_init")
+
+
+@pytest.mark.parametrize("channels", [5, 131, 260])
+def test_packed_in_place(channels):
+    offsets = offsets_of([90, 0, 200, 7], 11)
+    gate, x, init, _, _ = inputs(22, (330, channels), 4, F32, F32, True)
+    ref = Recurrence(gate, x, init, offsets, True)
+    for where in ("x", "gate"):
+        both = put(torch.cat([gate, x], -1))
+        g, v = both[..., :channels], both[..., channels:]
+        out = v if where == "x" else g
+        _, final = thrust_amd.linear_scan(g, v, init=put(init), offsets=put(offsets), log_gate=True, out=out)
+        got, was = get(out), x if where == "x" else gate
+        check(got[11:308], ref.out[0, 11:308], ref.error_out[0, 11:308], where)
+        assert torch.equal(got[:11], was[:11]) and torch.equal(got[308:], was[308:])
+        check(get(final), ref.final, ref.error_final, "final")
+
+
 def test_unaligned_views():
     shape = (1, 70, 135)
     gate, x, init, grad_out, grad_final = inputs(12, shape, 1, BF16, BF16, False)
@@ -396,6 +428,29 @@ def test_training_in_a_graph():
             one()  # eager work behind it
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.needs_device
+def test_step_in_a_graph():
+    gate, x, _, _, _ = inputs(42, (40, 1030), 40, F32, BF16, True)
+    state = torch.randn((64, 1030), generator=torch.Generator().manual_seed(8))
+    d = [put(t) for t in (gate, x, state)]
+    slots = put(torch.arange(40).int())
+    thrust_amd.linear_scan_step(d[0], d[1], d[2], slots=slots, log_gate=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = thrust_amd.linear_scan_step(d[0], d[1], d[2], slots=slots, log_gate=True)
+    g = torch.Generator().manual_seed(9)
+    for r in range(4):
+        new = torch.randint(-3, 64, (40,), generator=g).int()  # padded rows, and rows of one slot
+        slots.copy_(new)
+        d[2].copy_(state)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, after, error, error_state = step_reference(gate, x, state, new.tolist(), True)
+        check(get(out), want, error, "out")
+        check(get(d[2]), after, error_state, "state")
 
 
 @pytest.mark.needs_device

@@ -385,6 +385,31 @@ def test_requests_in_a_graph():
 
 
 @pytest.mark.needs_device
+def test_two_caches_on_two_streams():
+    pairs = [make(9000 if k else 300, [((64,), torch.float32)] * 3, 4, 200, 10, seed=k) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ids, lengths = list(range(100)), [(7 * i) % 41 for i in range(100)]
+    parents, children = list(range(0, 60, 3)), list(range(100, 120))
+    t = [ints(v) for v in (ids, lengths, parents, children, ids[:50])]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (cache, _), stream in zip(pairs, streams):
+            with torch.cuda.stream(stream):
+                cache.resize(t[0], t[1])
+                cache.fork(t[2], t[3])
+                cache.free(t[4])
+                cache.compact()
+    torch.cuda.synchronize()
+    for cache, ref in pairs:
+        for _ in range(3):
+            ref.resize(ids, lengths)
+            ref.fork(parents, children, True)
+            ref.free(ids[:50])
+            ref.compact()
+        same(cache, ref)
+
+
+@pytest.mark.needs_device
 def test_pools_past_4_gib():
     pages, width = 70000, 20000  # 5.6 GB of float32
     pool = torch.zeros((pages, width), device="cuda")
