@@ -204,9 +204,11 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  * rows, which the gradient needs.  out may be x or gate itself (same address, strides and type); any
  * other overlap of an output with an input is an error that is not detected.
  *
- * Infinities and NaNs stay in their channel and sequence.  Products of factors over up to 1024 rows are
- * formed on their own: where one underflows, an infinite state turns into NaN; where one overflows
- * 32 bits, a state of zero does.  Results are the same from run to run: what is combined with what
+ * Infinities and NaNs stay in their channel and sequence.  Products of factors have an exponent of their
+ * own: a state that is a normal number from row to row comes out as one, also where the product of the
+ * gates between leaves 32 bits; a state that leaves them on the way is 0 or infinite from there on.  What up
+ * to 1024 rows make of a state of zero is summed apart: where these terms alone overflow and only the
+ * state that enters would cancel them, the result is infinite or NaN.  Results are the same from run to run: what is combined with what
  * depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan; up to
  * THRUST_CDNA4_LINEAR_SCAN_CHUNK rows need none, and then only a non-null address and a size of 256.
  */

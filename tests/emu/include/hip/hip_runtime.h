@@ -246,6 +246,12 @@ inline unsigned emu_mbcnt_hi(unsigned mask, unsigned base) {
 #define __threadfence() __atomic_thread_fence(__ATOMIC_SEQ_CST)
 #define __threadfence_block() __atomic_thread_fence(__ATOMIC_SEQ_CST)
 #define __threadfence_system() __atomic_thread_fence(__ATOMIC_SEQ_CST)
+// the significand of [1/2, 1) and its exponent; zeros, infinities and NaNs stay as they are and have exponent 0
+inline float emu_frexp_mant(float v) { int e; return std::isfinite(v) ? std::frexp(v, &e) : v; }
+inline int emu_frexp_exp(float v) { int e = 0; if (std::isfinite(v)) std::frexp(v, &e); return e; }
+#define __builtin_amdgcn_frexp_mantf(v) emu_frexp_mant(v)
+#define __builtin_amdgcn_frexp_expf(v) emu_frexp_exp(v)
+#define __builtin_amdgcn_ldexpf(v, e) std::ldexp((float)(v), (int)(e))
 #define __builtin_amdgcn_s_sleep(n) ::emu::sleep()
 #define __builtin_amdgcn_s_setprio(n) ((void)0)
 #define __builtin_amdgcn_sched_barrier(n) ((void)0)

@@ -493,3 +493,70 @@ def test_no_wait_was_given_up():
     capi.check(capi.lib().thrust_cdna4_lookback_timeouts(ctypes.byref(count)), "lookback_timeouts")
     assert count.value == 0
     gpu_util.synchronize()
+
+
+# ---------------------------------------------------------------------------------------
+# Gates whose products leave the range of 32 bits where the states do not
+# ---------------------------------------------------------------------------------------
+# name: rows, {row: gate} (1 elsewhere), initial state, gradient of the final one.  Every state of the rows one after the other, and
+# every gradient, is a normal number of 32 bits; the product of some of the gates is not.
+RANGES = {
+    "over, along tiles": (900, {t: 2.0 for t in range(512, 640)}, 1e-20, 1e-20),
+    "under, along tiles": (900, {t: 0.5 for t in range(512, 672)}, 1e30, 1e30),
+    "over, along wavefronts": (70, {t: 64.0 for t in range(8, 38)}, 1e-25, 1e-25),
+    "under, along wavefronts": (70, {t: 2.0 ** -6 for t in range(8, 38)}, 1e25, 1e25),
+    "over, along rows": (5, {1: 1e20, 2: 1e20}, 1e-30, 1e-18),
+    "under, along rows": (5, {1: 1e-25, 2: 1e-20}, 1e30, 1e18),
+    "over and back": (1500, {**{t: 8.0 for t in range(100, 160)}, **{t: 0.125 for t in range(1300, 1350)}}, 1e-25, 1e20),
+    "under and back": (1500, {**{t: 0.125 for t in range(100, 160)}, **{t: 8.0 for t in range(1300, 1350)}}, 1e25, 1e-10),
+    "over and back in a wavefront": (16, {2: 1e18, 3: -1e18, 4: 1e18, 5: 1e-17, 6: 1e-18, 7: 1e-18}, 1e-27, 1e20),
+    "the smallest gate": (200, {150: 2.0 ** -133, 151: 0.5}, 1e30, 1e5),
+    "past a super-group": (9100, {t: 0.5 for t in range(8100, 8280)}, -1e35, 1e25),
+}
+
+
+@pytest.mark.parametrize("which", list(RANGES), ids=str)
+@pytest.mark.parametrize("gate_t,x_t,channels,log", [(F32, F32, 4, False), (BF16, BF16, 132, False), (F32, BF16, 132, True), (F32, F32, 130, False)], ids=name)
+def test_products_of_gates_out_of_range(which, gate_t, x_t, channels, log):
+    rows, gates, first, last = RANGES[which]
+    if channels > 4 and rows > 1600:
+        channels = 129
+    gate = torch.ones(1, rows, channels, dtype=torch.float64)
+    for t, a in gates.items():
+        gate[0, t] = a
+    if log:
+        gate = gate.abs().log()
+    gate = gate.to(gate_t)
+    x, grad_out = torch.zeros(1, rows, channels, dtype=x_t), torch.zeros(1, rows, channels, dtype=x_t)
+    scale = 1 + torch.arange(channels) / 512.0
+    init, grad_final = (first * scale)[None].float(), (last * scale)[None].float()
+    ref = Recurrence(gate, x, init, None, log).gradient(grad_out, grad_final)
+    for v in (ref.out, ref.grad_x, ref.grad_x * ref.a, ref.grad_x * ref.before, ref.grad_gate):  # what is said above
+        assert v.abs().min() >= 2.0 ** -126 and v.abs().max() < 2.0 ** 128
+    d = [put(t) for t in (gate, x, init, grad_out, grad_final)]
+    out, final, states = thrust_amd.linear_scan(d[0], d[1], init=d[2], log_gate=log, return_states=True)
+    check(get(out), ref.out, ref.error_out, "out")
+    check(get(final), ref.final, ref.error_final, "final")
+    grads = thrust_amd.linear_scan_backward(d[3], d[0], d[1], states, init=d[2], grad_final=d[4], log_gate=log)
+    check(get(grads[1]), ref.grad_x, ref.error_x, "grad_x")
+    check(get(grads[0]), ref.grad_gate, ref.error_gate, "grad_gate")
+    check(get(grads[2]), ref.grad_init, ref.error_init, "grad_init")
+    # the same as one of several packed sequences
+    offsets = offsets_of([70, rows, 0, 33]).int()
+    wide = (rows + 103, channels)
+    g, v = torch.full(wide, float(0 if log else 1)).to(gate_t), torch.ones(wide).to(x_t)
+    g[70:70 + rows], v[70:70 + rows] = gate[0], 0
+    starts = torch.ones(4, channels)
+    starts[1] = init[0]
+    out, final = forward(g, v, starts, offsets, log)
+    check(get(out)[70:70 + rows], ref.out[0], ref.error_out[0], "packed")
+    check(get(final)[1], ref.final[0], ref.error_final[0], "packed, final")
+
+
+def test_infinite_and_zero_states_meet_products_out_of_range():
+    """An infinite state stays infinite under gates that are not zero, and a zero one zero under finite ones."""
+    for a in (2.0 ** -6, 64.0):
+        gate, x = torch.full((1, 700, 4), a), torch.zeros(1, 700, 4)
+        out, final = forward(gate, x, torch.tensor([[float("inf"), 0.0, -float("inf"), float("nan")]]), None, False)
+        got = torch.cat([get(out)[0], get(final)])
+        assert (got[:, 0] == float("inf")).all() and (got[:, 1] == 0).all() and (got[:, 2] == -float("inf")).all() and got[:, 3].isnan().all()

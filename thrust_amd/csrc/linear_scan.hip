@@ -35,6 +35,10 @@
 // relaxed agent-scope atomic; NaNs are stored as the canonical one, so no map is the word 0, which
 // means "not there yet" and is what the clearing kernel leaves.
 //
+// Range.  A is a product of up to 1024 gates and leaves 32 bits where the states do not, so products have
+// exponents of their own; plain ones took 313.5 us instead of 322 for the long sequence, 380 instead of
+// 391 for the dense training pass.
+//
 // Sequences.  A row that begins a sequence takes its initial state by selection, never by a product
 // with zero, so infinities and NaNs of one sequence stay in it.  Which predecessors a tile needs
 // follows from the offsets alone, as does whether a published map begins anew.
@@ -79,10 +83,54 @@ struct LinArgs {
 // ---------------------------------------------------------------------------------------
 __device__ inline uint32_t canonical_bits(float v) { return v != v ? 0x7fc00000u : bit_cast<uint32_t>(v); }
 
-struct Map {
-  float a, h;
+// A product of factors, m 2^e, |m| < 1.  The product leaves the range of 32 bits where the states that it
+// takes one to the other do not (160 gates of one half and a state of 1e30), so it has an exponent of its own;
+// m is 0, infinite or NaN where a factor is.
+struct Product {
+  float m;
+  int e;
 };
-__device__ inline void publish_map(uint64_t* p, Map m) { st_agent(p, ~(((uint64_t)canonical_bits(m.a) << 32) | canonical_bits(m.h))); }
+__device__ inline void times(Product& p, float a) {
+  p.m *= __builtin_amdgcn_frexp_mantf(a);  // of [1/2, 1): 16 of them, and 24 that are normalised, stay in range
+  p.e += __builtin_amdgcn_frexp_expf(a);
+}
+__device__ inline Product normalised(Product p) {
+  return Product{__builtin_amdgcn_frexp_mantf(p.m), p.e + __builtin_amdgcn_frexp_expf(p.m)};
+}
+// An exponent out of [kLowest + 1, kHighest - 1] takes every finite state but 0 to 0, or to infinity, and
+// whatever follows leaves it there.
+constexpr int kLowest = -511, kHighest = 510;
+__device__ inline bool out_of_range(int e) { return (uint32_t)(e - kLowest - 1) >= (uint32_t)(kHighest - kLowest - 1); }
+// b after a
+__device__ inline Product join(Product a, Product b) { return Product{a.m * b.m, out_of_range(a.e) ? a.e : out_of_range(b.e) ? b.e : a.e + b.e}; }
+// a h + x for a normalised product a
+__device__ inline float apply(Product a, float h, float x) { return __builtin_amdgcn_ldexpf(a.m * h, a.e) + x; }
+
+// A published product has 32 bits: a sign, 10 of the exponent, 21 of the mantissa behind its leading 1.  The
+// two bits that a float has more go to the exponent; that costs 2^-22 relative, as much as four roundings of 32
+// bits, for a hop of 64 rows or more, each of which rounds twice.
+__device__ inline uint32_t product_bits(Product p) {
+  p = normalised(p);
+  const uint32_t u = bit_cast<uint32_t>(p.m), sign = u & 0x80000000u;
+  const uint32_t r = ((u & 0x7fffffffu) + 1u + (u >> 2 & 1u)) >> 2;  // to nearest, ties to even: 126 << 21 and on, or 127 << 21
+  int e = p.e + (int)(r >> 21) - 126;
+  e = e < kLowest ? kLowest : e > kHighest ? kHighest : e;
+  uint32_t v = (uint32_t)(e + 512) << 21 | (r & 0x1fffffu);  // 1 .. 1022 in the exponent's place
+  if (p.m == 0.f) v = 0;
+  if (!(__builtin_fabsf(p.m) < 1.f)) v = 1023u << 21 | (p.m != p.m ? 1u : 0u);
+  return sign | v;
+}
+__device__ inline Product product_of(uint32_t v) {
+  const uint32_t code = v >> 21 & 1023u;
+  const uint32_t exponent = code == 0 ? 0u : code == 1023 ? 255u << 23 : 126u << 23;
+  return Product{bit_cast<float>((v & 0x80000000u) | exponent | (v & 0x1fffffu) << 2), (int)code - 512};
+}
+
+struct Map {
+  Product a;
+  float h;
+};
+__device__ inline void publish_map(uint64_t* p, Map m) { st_agent(p, ~(((uint64_t)product_bits(m.a) << 32) | canonical_bits(m.h))); }
 
 // ---------------------------------------------------------------------------------------
 // Sequences of packed rows.  Everything here is the same in all lanes of a wavefront.  Offsets that
@@ -210,8 +258,10 @@ __device__ inline void store_state(float* p, int64_t row, uint32_t c, const floa
 // ---------------------------------------------------------------------------------------
 template <int CH>
 struct LinShared {
-  float a[kLinWaves][CH], h[kLinWaves][CH];  // maps of the tile's wavefronts
-  float map_a[CH], map_h[CH];                // the map of the group's earlier tiles
+  float m[kLinWaves][CH], h[kLinWaves][CH];  // maps of the tile's wavefronts, the factors normalised
+  int e[kLinWaves][CH];
+  float map_m[CH], map_h[CH];                // the map of the group's earlier tiles, likewise
+  int map_e[CH];
   float carry[CH];                           // the state before them
   int in_group;                              // the sequence begins among them: map_h is a state, and all there is
   int anew[kLinWaves];  // wavefront: a sequence begins in it (its h is then a state)
@@ -219,16 +269,24 @@ struct LinShared {
   uint32_t ticket;
 };
 
-// One channel: the maps m0, m0 + 1 .. m1 - 1 of (a, h) after (A, H)
+// One channel: the maps of the wavefronts w0, w0 + 1 .. w1 - 1 after (A, H)
 template <int CH>
-__device__ inline void fold(const float (*a)[CH], const float (*h)[CH], int m0, int m1, int ch, float& A, float& H) {
-  for (int m = m0; m < m1; m++) {
-    H = a[m][ch] * H + h[m][ch];
-    A *= a[m][ch];
+__device__ inline void fold(const LinShared<CH>& sm, int w0, int w1, int ch, Product& A, float& H) {
+  for (int w = w0; w < w1; w++) {
+    const Product a{sm.m[w][ch], sm.e[w][ch]};
+    H = apply(a, H, sm.h[w][ch]);
+    A.m *= a.m;
+    A.e += a.e;
   }
 }
-__device__ inline float map_factor(uint64_t word) { return bit_cast<float>((uint32_t)(~word >> 32)); }
+__device__ inline Product map_factor(uint64_t word) { return product_of((uint32_t)(~word >> 32)); }
 __device__ inline float map_shift(uint64_t word) { return bit_cast<float>((uint32_t)~word); }
+
+// The state behind the group's earlier tiles
+template <int CH>
+__device__ inline float group_state(const LinShared<CH>& sm, int ch) {
+  return sm.in_group ? sm.map_h[ch] : apply(Product{sm.map_m[ch], sm.map_e[ch]}, sm.carry[ch], sm.map_h[ch]);
+}
 
 // Waits until n words that start `stride` elements apart are published; they have been asked for once.
 template <int N, class W>
@@ -250,9 +308,9 @@ __device__ inline void wait_words(const W* p, int64_t stride, uint32_t c, W (&v)
   atomicAdd(&g_linear_scan_timeouts, 1u);
 }
 
-// Called by the whole workgroup after sm.a, sm.h, sm.anew and sm.since are written and a barrier.
+// Called by the whole workgroup after sm.m, sm.e, sm.h, sm.anew and sm.since are written and a barrier.
 // `i`: logical tile of `nt`; `rows`: rows of a tile.  Leaves the map of the group's earlier tiles in
-// sm.map_a and sm.map_h and the state before them in sm.carry.  One half of the workgroup deals with the
+// sm.map_m, sm.map_e and sm.map_h and the state before them in sm.carry.  One half of the workgroup deals with the
 // tiles of the group and the other with what lies before it, a thread for each channel; what a thread
 // may wait for it asks for at once, so that maps which are there cost one trip to memory.
 template <int VEC>
@@ -275,13 +333,15 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
   last_anew = __builtin_amdgcn_readfirstlane(last_anew);
   // the tile's own map after (A, H); folded again where it is needed again, which is rare, rather than
   // kept in registers over the waits
-  auto tile_after = [&](float A, float H) {
+  auto tile_after = [&](Product A, float H) {
+    Product own{1.f, 0};
     if (last_anew >= 0) H = sm.h[last_anew][ch];
-    fold<CH>(sm.a, sm.h, last_anew + 1, kLinWaves, ch, A, H);
-    return Map{A, H};
+    fold<CH>(sm, last_anew + 1, kLinWaves, ch, own, H);
+    return Map{join(A, own), H};
   };
+  const Product one{1.f, 0};
   if (role == 0 && from < C) {
-    if (publishes) publish_map(at(p.tile_map + ((int64_t)b * nt + i) * C, chan), tile_after(1.f, 0.f));
+    if (publishes) publish_map(at(p.tile_map + ((int64_t)b * nt + i) * C, chan), tile_after(one, 0.f));
     __builtin_amdgcn_sched_barrier(0);  // the folded maps' registers are free for the words that follow
     const uint64_t* maps = p.tile_map + ((int64_t)b * nt + base) * C;
     const int k0 = needs ? (int)(in_group ? first - base : 0) : N, k1 = (int)(i - base);
@@ -290,18 +350,22 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
     for (int k = 0; k < N; k++) v[k] = k >= k0 && k < k1 ? ld_agent(at(maps + k * C, chan)) : ~uint64_t(0);
     wait_words(maps, C, chan, v);
     // (GA, GH): the map of the group's earlier tiles, or GH a state where the sequence begins among them
-    float GA = 1.f, GH = 0.f;
+    Product GA = one;
+    float GH = 0.f;
 #pragma unroll
     for (int k = 0; k < N; k++) {
       if (k >= k0 && k < k1) {
-        const float a = map_factor(v[k]), h = map_shift(v[k]);
-        GH = in_group && k == k0 ? h : a * GH + h;
-        GA = in_group && k == k0 ? 0.f : GA * a;
+        const Product a = map_factor(v[k]);
+        const float h = map_shift(v[k]);
+        GH = in_group && k == k0 ? h : apply(a, GH, h);
+        GA = join(GA, a);
       }
     }
     if (publishes && i - base == N)
       publish_map(at(p.group_map + ((int64_t)b * groups + g) * C, chan), tile_after(GA, GH));
-    sm.map_a[ch] = GA;
+    GA = normalised(GA);
+    sm.map_m[ch] = GA.m;
+    sm.map_e[ch] = GA.e;
     sm.map_h[ch] = GH;
   } else if (role == 1 && from < C) {
     float H = 0.f;
@@ -321,8 +385,8 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
 #pragma unroll
       for (int k = 0; k < N; k++) {
         if (k >= k0 && k < k1) {
-          const float a = map_factor(v[k]), h = map_shift(v[k]);
-          H = !from_super && k == k0 ? h : a * H + h;
+          const float h = map_shift(v[k]);
+          H = !from_super && k == k0 ? h : apply(map_factor(v[k]), H, h);
         }
       }
     }
@@ -331,8 +395,8 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
   if (threadIdx.x == 0) sm.in_group = in_group;
   __syncthreads();
   if (role == 0 && from < C && publishes && i % kLinSuper == kLinSuper - 1) {
-    const float H = in_group ? sm.map_h[ch] : sm.map_a[ch] * sm.carry[ch] + sm.map_h[ch];
-    st_agent(at(p.super_state + ((int64_t)b * supers + sg) * C, chan), ~canonical_bits(tile_after(1.f, H).h));
+    const float H = group_state(sm, ch);
+    st_agent(at(p.super_state + ((int64_t)b * supers + sg) * C, chan), ~canonical_bits(tile_after(one, H).h));
   }
 }
 
@@ -346,9 +410,9 @@ __device__ inline void wave_carry(const LinShared<kWave * VEC>& sm, int lw, int 
 #pragma unroll
   for (int j = 0; j < VEC; j++) {
     const int ch = lane * VEC + j;
-    float A = 1.f;
-    h[j] = last_anew >= 0 ? sm.h[last_anew][ch] : sm.in_group ? sm.map_h[ch] : sm.map_a[ch] * sm.carry[ch] + sm.map_h[ch];
-    fold<kWave * VEC>(sm.a, sm.h, last_anew + 1, lw, ch, A, h[j]);
+    Product A{1.f, 0};
+    h[j] = last_anew >= 0 ? sm.h[last_anew][ch] : group_state(sm, ch);
+    fold<kWave * VEC>(sm, last_anew + 1, lw, ch, A, h[j]);
   }
 }
 
@@ -440,7 +504,7 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
     gates_of_logarithms<TG, VEC, S>(p, gate);
   }
   auto gate_value = [&](const Pack<TG, VEC>& g, int j) { return LOG16 ? expf(g.value(j)) : g.value(j); };
-  auto step = [&](int k, float (&h)[VEC], float (&A)[VEC], int& s) {
+  auto step = [&](int k, float (&h)[VEC], Product (&A)[VEC], int& s) {
     if (span.heads >> k & 1) {
       to_sequence<PACKED>(p, span, begins[PACKED ? w : 0], r0, k, s);
       load_state<VEC>(p.init, (int64_t)s * C, c0, h);
@@ -449,19 +513,22 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
     for (int j = 0; j < VEC; j++) {
       const float a = gate_value(gate[k], j);
       h[j] = a * h[j] + x[k].value(j);
-      A[j] *= a;
+      times(A[j], a);
     }
   };
-  float h[VEC], A[VEC];
+  float h[VEC];
+  Product A[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = 1.f;
+  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = Product{1.f, 0};
   int s = span.first_sequence;
 #pragma unroll
   for (int k = 0; k < S; k++)
     if (span.inside >> k & 1) step(k, h, A, s);
 #pragma unroll
   for (int j = 0; j < VEC; j++) {
-    sm.a[w][lane * VEC + j] = A[j];
+    const Product a = normalised(A[j]);
+    sm.m[w][lane * VEC + j] = a.m;
+    sm.e[w][lane * VEC + j] = a.e;
     sm.h[w][lane * VEC + j] = h[j];
   }
   if (lane == 0) sm.anew[w] = span.heads != 0;
@@ -482,8 +549,9 @@ __global__ __launch_bounds__(kLinBlock) void linear_scan_kernel(LinArgs p) {
   wave_carry<VEC>(sm, w, lane, h);
   s = span.first_sequence;
   if (p.states && left > 0 && r0 % kLinChunk == 0 && active) {
-    if (span.heads & 1) load_state<VEC>(p.init, (int64_t)s * C, c0, A);
-    store_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + r0 / kLinChunk) * C, c0, span.heads & 1 ? A : h);
+    float first[VEC];
+    if (span.heads & 1) load_state<VEC>(p.init, (int64_t)s * C, c0, first);
+    store_state<VEC>(p.states, (b * ceil_div(p.rows, (int64_t)kLinChunk) + r0 / kLinChunk) * C, c0, span.heads & 1 ? first : h);
   }
   TX* out = static_cast<TX*>(p.out) + b * p.out_bs + r0 * p.out_rs;
 #pragma unroll
@@ -568,9 +636,10 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
       load_state<VEC>(p.grad_final, (int64_t)s * C, c0, c);
     }
   };
-  float A[VEC], c[VEC];
+  Product A[VEC];
+  float c[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = 1.f, c[j] = 0.f;
+  for (int j = 0; j < VEC; j++) h[j] = 0.f, A[j] = Product{1.f, 0}, c[j] = 0.f;
   int s = span.first_sequence;
 #pragma unroll
   for (int k = 0; k < S; k++) {
@@ -580,7 +649,7 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
       for (int j = 0; j < VEC; j++) {
         const float a = gate_value(gate[k], j);
         h[j] = a * h[j] + x[k].value(j);
-        A[j] *= a;
+        times(A[j], a);
       }
     }
   }
@@ -595,7 +664,9 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
   }
 #pragma unroll
   for (int j = 0; j < VEC; j++) {
-    sm.a[lw][lane * VEC + j] = A[j];
+    const Product a = normalised(A[j]);
+    sm.m[lw][lane * VEC + j] = a.m;
+    sm.e[lw][lane * VEC + j] = a.e;
     sm.h[lw][lane * VEC + j] = c[j];
     fwd[w][lane * VEC + j] = h[j];
     if (w == 0) entering[lane * VEC + j] = enter[j];
@@ -636,7 +707,7 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
     for (int j = 0; j < VEC; j++) {
       const int ch = lane * VEC + j;
       h[j] = last_anew >= 0 ? fwd[last_anew][ch] : entering[ch];
-      for (int v = last_anew + 1; v < w; v++) h[j] = sm.a[kLinWaves - 1 - v][ch] * h[j] + fwd[v][ch];
+      for (int v = last_anew + 1; v < w; v++) h[j] = apply(Product{sm.m[kLinWaves - 1 - v][ch], sm.e[kLinWaves - 1 - v][ch]}, h[j], fwd[v][ch]);
     }
   }
   float before[S][VEC];
