@@ -280,11 +280,12 @@ int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, con
  * [num_sequences][max_pages], -1 behind a sequence's pages.  A length is a number of tokens; a sequence
  * of length n holds the first ceil(n / page_size) entries of its row.
  *
- * Requests of a call are served as if in their order: each in turn takes the lowest free pages.  One
- * that cannot be served leaves everything of its sequence as it was and has done[i] = 0, and so has
- * one with an id out of range or a sequence that an earlier request of the call names already.  One
- * that needs pages is refused when the pages wanted by it and by all requests before it (refused ones
- * among them) are more than there were free.  Entries of a table that name no page are passed over.
+ * Requests of a call are served in their order: each in turn takes the lowest free pages, with the counts
+ * as those before it left them.  One that cannot be served leaves everything of its sequence as it was and
+ * has done[i] = 0, and so has one with an id out of range or a sequence that an earlier request of the call
+ * names already.  What a refused request wanted stays out of reach for the rest of the call: one that
+ * needs pages is refused when the pages wanted by it and by all requests before it (refused ones among
+ * them) are more than there were free.  Entries of a table that name no page are passed over.
  */
 typedef struct thrust_cdna4_page_cache {
   const uint64_t* pools;
@@ -307,7 +308,8 @@ int thrust_cdna4_pages_fork(void* temp, size_t* temp_bytes, const thrust_cdna4_p
  * sequences[i] gets the length lengths[i].  Pages that shrinking
  * sequences give up are there for the growing ones of the same call.  A growing sequence whose last
  * page is partly filled and named by others too gets a copy of that page, so that what is appended is
- * its own.  A length that is negative or over max_pages * page_size is refused.
+ * its own; if all that name it grow in the call, the last of them is alone with it by then and keeps it.  A
+ * length that is negative or over max_pages * page_size is refused.
  */
 int thrust_cdna4_pages_resize(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, const int32_t* sequences,
                               const int32_t* lengths, int64_t n, uint8_t* done, void* stream);

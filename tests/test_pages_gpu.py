@@ -425,3 +425,120 @@ def test_pools_past_4_gib():
     assert get(cache.tables)[:2, 0].tolist() == [6, 5]
     want = torch.arange(width).float()
     assert torch.equal(get(pool[5]), want) and torch.equal(get(pool[6]), want)
+
+
+# ---------------------------------------------------------------------------------------
+# Growth into pages that are shared, request after request
+# ---------------------------------------------------------------------------------------
+class InOrder(Lists):
+    """As Lists, with the counts as the requests before left them: who is alone with its page when its turn comes keeps it."""
+
+    def resize(self, sequences, lengths, free_only=False):
+        ok = super().resize(sequences, [min(a, self.lengths[s]) if self.valid(s) and a >= 0 else a for s, a in zip(sequences, lengths)], free_only)
+        if free_only:
+            return ok
+        free, at, copies = [p for p, r in enumerate(self.refs) if r == 0], 0, []
+        for i, (s, want) in enumerate(zip(sequences, lengths)):
+            ok[i] = ok[i] and want <= self.most * self.size
+            if not ok[i] or want <= self.lengths[s]:
+                continue
+            had, part = self.held(self.lengths[s]), self.lengths[s] % self.size
+            last = self.tables[s][had - 1] if part else -1
+            own = 0 <= last < len(self.refs) and self.refs[last] > 1
+            need = self.held(want) - had + own
+            mine = free[at:at + need]
+            at += need
+            if len(mine) < need:
+                ok[i] = False
+                continue
+            if own:
+                copies.append((last, mine[0]))
+                self.refs[last] -= 1
+                self.refs[mine[0]] = 1
+                self.tables[s][had - 1] = mine.pop(0)
+            for j, p in enumerate(mine):
+                self.tables[s][had + j], self.refs[p] = p, 1
+            self.lengths[s] = want
+        self.copy(copies)
+        return ok
+
+
+def shared(pages, sequences, page_size, most, groups, unused=0):
+    """A cache in which the sequences of a group share the first pages of its first one, cut back into the last of them."""
+    cache, ref = make(pages, [((page_size, 3), torch.float32), ((page_size, 3), torch.int32)], page_size, sequences, most)
+    ref.__class__ = InOrder
+    for members, full, keep in groups:
+        for c, v in ((cache, ints), (ref, lambda x: x)):
+            c.resize(v(members[:1]), v([full * page_size]))
+            for k in range(1, len(members)):
+                if c is cache:
+                    c.fork(v(members[:1]), v(members[k:k + 1]))
+                else:
+                    c.fork(members[:1], members[k:k + 1], True)
+            c.resize(v(members), v([keep] * len(members)))
+    same(cache, ref)
+    return cache, ref
+
+
+def test_the_last_of_those_that_grow_keeps_the_page():
+    cache, ref = shared(3, 2, 4, 2, [([0, 1], 2, 6)])
+    assert get(cache.resize(ints([0, 1]), ints([7, 7]))).tolist() == [True, True] == ref.resize([0, 1], [7, 7])
+    assert get(cache.tables).tolist() == [[0, 2], [0, 1]] and get(cache.refs).tolist() == [2, 1, 1]
+    same(cache, ref)
+    # one that does not grow keeps it too; of three that grow two are given copies
+    cache, ref = shared(9, 4, 4, 4, [([2, 0, 3, 1], 1, 3)])
+    assert get(cache.resize(ints([3, 0, 1]), ints([4, 9, 1]))).tolist() == [True] * 3 == ref.resize([3, 0, 1], [4, 9, 1])
+    same(cache, ref)
+    assert get(cache.refs).tolist() == [2, 1, 1, 1, 1, 0, 0, 0, 0]
+    assert get(cache.resize(ints([1, 2]), ints([5, 4]))).tolist() == [True] * 2 == ref.resize([1, 2], [5, 4])
+    same(cache, ref)
+
+
+def test_a_page_is_not_kept_where_one_before_was_refused():
+    # sequence 0 would leave the page but finds no copy: sequence 1 still shares it and is refused too, 4 is served
+    groups = [([0, 1], 1, 2), ([2], 2, 8), ([3], 1, 4), ([4], 1, 1)]
+    cache, ref = shared(5, 5, 4, 4, groups)
+    assert get(cache.resize(ints([0, 1, 4]), ints([3, 3, 2]))).tolist() == [False, False, True] == ref.resize([0, 1, 4], [3, 3, 2])
+    same(cache, ref)
+    # an unrelated request between them is refused: the second of the two keeps the page all the same
+    cache, ref = shared(6, 5, 4, 4, groups)
+    for c, v in ((cache, ints), (ref, list)):
+        done = c.resize(v([0, 3, 1, 4, 2]), v([3, 9, 3, 4, 8]))
+        assert (get(done).tolist() if c is cache else done) == [True, False, True, True, True]
+    same(cache, ref)
+    # it wants pages besides: refused with the rest
+    cache, ref = shared(7, 5, 4, 4, groups)
+    for c, v in ((cache, ints), (ref, list)):
+        done = c.resize(v([0, 1, 3]), v([3, 16, 5]))
+        assert (get(done).tolist() if c is cache else done) == [True, False, False]
+    same(cache, ref)
+
+
+@pytest.mark.parametrize("pages,sequences,requests", [(60, 24, 20), (400, 150, 64), (400, 150, 65), (700, 300, 290), (9000, 60, 50)], ids=str)
+def test_many_that_grow_into_shared_pages(pages, sequences, requests):
+    rng = random.Random(requests)
+    size, most = 4, 6
+    for turn in range(4):
+        ids, groups = list(range(sequences)), []
+        rng.shuffle(ids)
+        room = pages // 2
+        while ids and room >= 5:
+            members = [ids.pop() for _ in range(min(len(ids), rng.choice([1, 2, 3, 9, 40])))]
+            full = rng.randint(1, 4)
+            groups.append((members, full, rng.randint(1, full * size)))
+            room -= full
+        cache, ref = shared(pages, sequences, size, most, groups)
+        if turn % 2:  # few pages are left
+            spare = ref.refs.count(0) - rng.randint(0, sequences // 2)
+            for c in (cache.refs, None):
+                held = [p for p, r in enumerate(ref.refs) if r == 0][:spare]
+                if c is not None:
+                    c[put(torch.tensor(held, dtype=torch.int64))] = 1
+            for p in held:
+                ref.refs[p] = 1
+        names = rng.sample(range(sequences), min(requests, sequences))
+        names[0], names[-1] = names[-1], names[1]  # one twice
+        lengths = [max(0, min(size * most + 1, ref.lengths[s] + rng.choice([0, 1, 1, 1, 1, 2, 7, -3]))) for s in names]
+        done = get(cache.resize(ints(names), ints(lengths))).tolist()
+        assert done == ref.resize(names, lengths)
+        same(cache, ref)

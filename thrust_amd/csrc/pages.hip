@@ -44,7 +44,8 @@ struct PageTemp {
   int32_t* span_free;  // free pages of each span
   int32_t* need;       // pages a request wants; -1: refused
   int64_t* start;      // pages wanted by the requests before it
-  int32_t* copied;     // resize: the page that a growing sequence gets a copy of; -1: none
+  int32_t* copied;     // resize: the page that a growing sequence gets a copy of; -1: none; -2 - j: it keeps a shared
+                       // page if request j, the last one that leaves it, is served
   int32_t* free_list;  // free pages, ascending; a compaction's holes
   int32_t* movers;     // a compaction's pages that move, descending, and their counts
   int32_t* mover_refs;
@@ -236,18 +237,48 @@ __global__ __launch_bounds__(kPageBlock) void pages_shrink_kernel(PageCache c, P
   if (i < r.n) shrink(c, t, r, i);
 }
 
-// the last page of a growing sequence when others name it too and something of it is free
-__device__ inline int page_to_copy(const PageCache& c, int s, int old, int want) {
+// The last page of a growing sequence when others name it too and something of it is free.  Requests are
+// served in their order: each that grows into a page gets a copy and leaves it, until the one whose turn
+// comes is alone with it and keeps it.  So with n names before the call, the n-th that grows into it keeps it;
+// but for that all before it must be served, and those which copy are refused from one on.
+__device__ inline int shared_page(const PageCache& c, int s, int old, int want) {
   if (want <= old || old % c.page_size == 0) return -1;
   const int q = c.tables[(int64_t)s * c.max_pages + old / c.page_size];
   return is_page(c, q) && c.refs[q] > 1 ? q : -1;
 }
 
-// What a valid resize wants; sets the page that it copies.
-__device__ inline int wanted_by_resize(const PageCache& c, const Requests& r, int64_t i, int32_t& copied) {
-  const int s = r.named[i], old = clamped_length(c, s), want = r.first[i];
-  copied = page_to_copy(c, s, old, want);
+__device__ inline int shared_page(const PageCache& c, const Requests& r, int64_t i) {
+  return shared_page(c, r.named[i], clamped_length(c, r.named[i]), r.first[i]);
+}
+// What becomes of it: `before` requests grow into it earlier in the call, the last of them `last`.
+__device__ inline int copied_page(const PageCache& c, int q, int before, int last) {
+  return q < 0 ? -1 : before < c.refs[q] - 1 ? q : -2 - last;
+}
+// What a valid resize wants
+__device__ inline int wanted_by_resize(const PageCache& c, const Requests& r, int64_t i, int copied) {
+  const int old = clamped_length(c, r.named[i]), want = r.first[i];
   return want <= old ? 0 : pages_of(c, want) - pages_of(c, old) + (copied >= 0);
+}
+// The same by a wavefront for one of many requests.  need[j] is replaced meanwhile by what request j wants, but
+// stays -1 where it is refused.
+__device__ inline bool refused(const PageTemp& t, int64_t j) { return (int)ld_agent(reinterpret_cast<const uint32_t*>(t.need + j)) < 0; }
+__device__ inline void plan_resize(const PageCache& c, const PageTemp& t, const Requests& r, int64_t i) {
+  if (refused(t, i)) return;
+  const int q = __builtin_amdgcn_readfirstlane(shared_page(c, r, i));
+  int before = 0, last = -1;
+  if (q >= 0) {  // rare: a sequence was cut back into what it shares
+    for (int64_t j0 = 0; j0 < i; j0 += kWave) {
+      const int64_t j = j0 + lane_id();
+      const uint64_t same = __ballot(j < i && !refused(t, j) && shared_page(c, r, j) == q);
+      before += __popcll(same);
+      if (same) last = (int)(j0 + kWave - 1 - __builtin_clzll(same));
+    }
+  }
+  if (lane_id() == 0) {
+    const int copied = copied_page(c, q, before, last);
+    t.copied[i] = copied;
+    st_agent(reinterpret_cast<uint32_t*>(t.need + i), (uint32_t)wanted_by_resize(c, r, i, copied));
+  }
 }
 // What a fork wants that names its child first and no parent as child; -1: refused.
 __device__ inline int wanted_by_fork(const PageCache& c, int kind, int parent, int child) {
@@ -262,13 +293,11 @@ __device__ inline bool valid_fork(const PageCache& c, int parent, int child) {
 // Tallies the free pages and what each request wants.
 __global__ __launch_bounds__(kPageBlock) void pages_tally_kernel(PageCache c, PageTemp t, Requests r) {
   if ((int)blockIdx.x < t.spans) return tally_span(c, t, (int)blockIdx.x);
-  const int64_t block = blockIdx.x - t.spans;
+  const int64_t i = (int64_t)(blockIdx.x - t.spans) * kRequestWaves + threadIdx.x / kWave;  // a wavefront for a request
+  if (i >= r.n) return;
   if (r.kind == kResize) {
-    const int64_t i = block * kPageBlock + threadIdx.x;
-    if (i < r.n && t.need[i] >= 0) t.need[i] = wanted_by_resize(c, r, i, t.copied[i]);
+    plan_resize(c, t, r, i);
   } else {
-    const int64_t i = block * kRequestWaves + threadIdx.x / kWave;  // a wavefront for a request
-    if (i >= r.n) return;
     const int parent = r.first[i], child = r.named[i];
     const bool ok = valid_fork(c, parent, child) && !named_before(r.named, i, child) && !named_before(r.first, r.n, child);
     if (lane_id() == 0) t.need[i] = ok ? wanted_by_fork(c, r.kind, parent, child) : -1;
@@ -338,10 +367,24 @@ __global__ __launch_bounds__(kSmallBlock) void pages_plan_small_kernel(PageCache
     __syncthreads();
   }
   int need = i < n ? s_need[i] : 0;
-  if (i < n) {
-    if (r.kind == kResize && need == 0) need = wanted_by_resize(c, r, i, t.copied[i]);
-    t.need[i] = need;
+  if (r.kind == kResize && w == 0) {
+    const bool valid = i < n && need == 0;
+    const int q = valid ? shared_page(c, r, i) : -1;
+    int before = 0, last = -1;
+    if (__ballot(q >= 0)) {
+      for (int j = 0; j < n; j++) {
+        const bool same = __builtin_amdgcn_readlane(q, j) == q && j < i;
+        before += same;
+        if (same) last = j;
+      }
+    }
+    if (valid) {
+      const int copied = copied_page(c, q, before, last);
+      t.copied[i] = copied;
+      need = wanted_by_resize(c, r, i, copied);
+    }
   }
+  if (i < n) t.need[i] = need;
   int64_t wanted;
   const int64_t start = block_exclusive(sm, (int64_t)(need > 0 ? need : 0), wanted);
   if (i < n) t.start[i] = start;
@@ -389,7 +432,9 @@ __global__ __launch_bounds__(kPageBlock) void pages_serve_kernel(PageCache c, Pa
   const int piece = (int)(blockIdx.x % (unsigned)pieces);
   const int need = t.need[i];
   const int64_t start = t.start[i];
-  const bool ok = need == 0 || (need > 0 && start + need <= t.head[1]);
+  const auto served = [&](int need, int64_t start) { return need == 0 || (need > 0 && start + need <= t.head[1]); };
+  bool ok = served(need, start);
+  if (ok && r.kind == kResize && t.copied[i] <= -2) ok = served(t.need[-2 - t.copied[i]], t.start[-2 - t.copied[i]]);
   if (piece == 0 && threadIdx.x == 0 && r.done) r.done[i] = ok;
   if (!ok) return;
   const int32_t* mine = t.free_list + start;
@@ -574,7 +619,7 @@ static hipError_t serve(const PageCache& c, const PageTemp& t, const Requests& r
   }
   if (r.kind == kResize)
     TCD_LAUNCH("pages_shrink_kernel", pages_shrink_kernel, dim3((unsigned)ceil_div(r.n, (int64_t)kRequestWaves)), dim3(kPageBlock), s, c, t, r);
-  const int64_t request_blocks = r.kind == kResize ? ceil_div(r.n, (int64_t)kPageBlock) : ceil_div(r.n, (int64_t)kRequestWaves);
+  const int64_t request_blocks = ceil_div(r.n, (int64_t)kRequestWaves);
   TCD_LAUNCH("pages_tally_kernel", pages_tally_kernel, dim3((unsigned)(t.spans + request_blocks)), dim3(kPageBlock), s, c, t, r);
   TCD_LAUNCH("pages_list_kernel", pages_list_kernel, dim3((unsigned)t.spans + 1u), dim3(kPageBlock), s, c, t, r.n);
   return grant(c, t, r, s);

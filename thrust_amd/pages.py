@@ -76,8 +76,8 @@ class PageCache:
 
     def resize(self, sequences, lengths):
         """sequences[i] gets the length lengths[i] (int32 tensors).  Pages given up are there for the
-        sequences that grow; one that grows into a page which others name too gets its own copy of it.
-        Returns bool [n]: False where a request was refused (an id out of range, a sequence named
+        sequences that grow; one that grows into a page which others name too gets its own copy of it
+        (requests are served in their order: if all of them grow, the last one keeps it).  Returns bool [n]: False where a request was refused (an id out of range, a sequence named
         before, a length out of range, not enough free pages), which changes nothing of the sequence."""
         n = self._requests(sequences, lengths)
         L = capi.lib()
