@@ -560,3 +560,23 @@ def test_infinite_and_zero_states_meet_products_out_of_range():
         out, final = forward(gate, x, torch.tensor([[float("inf"), 0.0, -float("inf"), float("nan")]]), None, False)
         got = torch.cat([get(out)[0], get(final)])
         assert (got[:, 0] == float("inf")).all() and (got[:, 1] == 0).all() and (got[:, 2] == -float("inf")).all() and got[:, 3].isnan().all()
+
+
+def test_torch_is_told_what_is_written():
+    """A tensor saved for somebody's backward pass and then written by a call is found out, as after any operation of torch in place."""
+    gate, x, init, _, _ = inputs(60, (2, 30, 5), 2, F32, F32, False)
+    g, v, state = put(gate), put(x), put(init)
+    weight = put(torch.ones(5)).requires_grad_()
+    loss = (v * weight).sum()
+    was = g._version, v._version
+    thrust_amd.linear_scan(g, v, out=v)
+    assert g._version == was[0] and v._version > was[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = (state * weight).sum()
+    rows, out = put(gate[:, 0]), put(x[:, 0])
+    was = rows._version, state._version, out._version
+    thrust_amd.linear_scan_step(rows, out, state, out=out)
+    assert rows._version == was[0] and state._version > was[1] and out._version > was[2]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -192,3 +192,27 @@ def test_refused_with_a_value_error(any_device, what):
     # (a cache's own check of requests compares devices, which are host ones here)
     with pytest.raises(ValueError):
         SCANS[what]()
+
+
+def test_a_forward_gradient_is_not_dropped(any_device):
+    """A dual tensor does not want a gradient of its own, and its tangent would be lost."""
+    from torch.autograd import forward_ad
+    x, state = Z(1, 5, 3), Z(5, 3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        flat, two = forward_ad.make_dual(Z(5, 3), torch.ones(5, 3)), forward_ad.make_dual(Z(1, 3), torch.ones(1, 3))
+        for call in (lambda: thrust_amd.linear_scan(dual, x), lambda: thrust_amd.linear_scan(x, dual), lambda: thrust_amd.linear_scan(x, x, init=two),
+                     lambda: thrust_amd.linear_scan(x, x, out=dual),
+                     lambda: thrust_amd.linear_scan_backward(dual, x, x, Z(1, 1, 3)), lambda: thrust_amd.linear_scan_backward(x, x, x, Z(1, 1, 3), grad_final=two),
+                     lambda: thrust_amd.linear_scan_step(flat, state, Z(5, 3)), lambda: thrust_amd.linear_scan_step(state, state, flat)):
+            for mode in (torch.enable_grad, torch.no_grad):  # which says nothing of forward mode
+                with mode(), pytest.raises(ValueError, match="differentiation"):
+                    call()
+
+
+def test_an_output_that_wants_its_gradient_is_refused(any_device):
+    x = Z(1, 5, 3)
+    with pytest.raises(ValueError, match="differentiation"):
+        thrust_amd.linear_scan(x, x, out=Z(1, 5, 3).requires_grad_())
+    with pytest.raises(ValueError, match="differentiation"):
+        thrust_amd.linear_scan_step(x[0], x[0], Z(5, 3), out=Z(5, 3).requires_grad_())

@@ -542,3 +542,22 @@ def test_many_that_grow_into_shared_pages(pages, sequences, requests):
         done = get(cache.resize(ints(names), ints(lengths))).tolist()
         assert done == ref.resize(names, lengths)
         same(cache, ref)
+
+
+def test_torch_is_told_what_is_written():
+    cache, _ = make(9, POOLS["keys and values"], 4, 5, 3)
+    own = [cache.tables, cache.lengths, cache.refs]
+
+    def written(call, tensors, kept=()):
+        was = [t._version for t in tensors], [t._version for t in kept]
+        call()
+        assert all(t._version > a for t, a in zip(tensors, was[0])) and [t._version for t in kept] == was[1]
+    written(lambda: cache.resize(ints([0, 1]), ints([5, 6])), own + cache.pools)
+    written(lambda: cache.fork(ints([0]), ints([2])), own + cache.pools)
+    written(lambda: cache.free(ints([1])), own, cache.pools)
+    written(lambda: cache.compact(), [cache.tables, cache.refs] + cache.pools, [cache.lengths])
+    apart = [put(torch.zeros_like(get(t))) for t in (cache.tables, cache.refs)]
+    written(lambda: cache.compact(*apart), apart + cache.pools, own)
+    with torch.inference_mode():  # tensors without a version
+        cache, _ = make(9, POOLS["keys and values"], 4, 5, 3)
+    cache.resize(ints([0, 1]), ints([5, 6]))

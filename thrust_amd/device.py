@@ -5,6 +5,7 @@ it can do without."""
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = contextlib.nullcontext()
 
@@ -51,7 +52,16 @@ def pointer(t):
 
 
 def no_autograd(*tensors):
-    """These calls are no nodes of torch's graph: a tensor that wants its gradient is not dropped in silence."""
+    """These calls are no nodes of torch's graph: a tensor that wants its gradient, or brings a tangent, is not dropped in silence."""
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError("no automatic differentiation: call under torch.no_grad(), with linear_scan_backward as the gradient")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("no automatic differentiation in forward mode")
+
+
+def wrote(tensors):
+    """Tells torch that a call has written to these, as its own operations in place do."""
+    torch._C._increment_version(tensors)

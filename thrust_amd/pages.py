@@ -47,6 +47,8 @@ class PageCache:
                                         tables=self.tables.data_ptr(), lengths=self.lengths.data_ptr(), refs=self.refs.data_ptr())
         self._ref = ctypes.byref(self._args)
         self._sizes = {}
+        self._own = [self.tables, self.lengths, self.refs]
+        self._all = self._own + pools
 
     def _array(self, given, shape, value, what):
         if given is None:
@@ -86,6 +88,7 @@ class PageCache:
             temp, nbytes = self._temp(L.thrust_cdna4_pages_resize, ("pages_resize", n), None, None, n, None)
             capi.check(L.thrust_cdna4_pages_resize(temp.data_ptr(), nbytes, self._ref, sequences.data_ptr(), lengths.data_ptr(), n,
                                                    done.data_ptr(), dev.stream(self.device)), "pages_resize")
+        dev.wrote(self._all)
         return done
 
     def free(self, sequences):
@@ -93,6 +96,7 @@ class PageCache:
         n = self._requests(sequences)
         with dev.current(self.device):
             capi.check(capi.lib().thrust_cdna4_pages_free(self._ref, sequences.data_ptr(), n, None, dev.stream(self.device)), "pages_free")
+        dev.wrote(self._own)
 
     def fork(self, parents, children, share=True):
         """Sequence children[i], which must be empty and no parent in the call, becomes a copy of
@@ -106,6 +110,7 @@ class PageCache:
             temp, nbytes = self._temp(L.thrust_cdna4_pages_fork, ("pages_fork", n), None, None, n, 0, None)
             capi.check(L.thrust_cdna4_pages_fork(temp.data_ptr(), nbytes, self._ref, parents.data_ptr(), children.data_ptr(), n, bool(share),
                                                  done.data_ptr(), dev.stream(self.device)), "pages_fork")
+        dev.wrote(self._all)
         return done
 
     def compact(self, tables=None, refs=None):
@@ -124,4 +129,5 @@ class PageCache:
             temp, nbytes = self._temp(L.thrust_cdna4_pages_compact, ("pages_compact",), None, None, None)
             capi.check(L.thrust_cdna4_pages_compact(temp.data_ptr(), nbytes, self._ref, tables.data_ptr(), refs.data_ptr(), live.data_ptr(),
                                                     dev.stream(self.device)), "pages_compact")
+        dev.wrote([tables, refs, *self.pools])
         return live

@@ -94,8 +94,9 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     or gate.  return_states: also the state that enters each chunk of 64 rows, for linear_scan_backward.
     Packed rows that belong to no sequence are left as they were in a given `out`, and zero in a new one."""
     device = dev.need_device(gate, x, init, offsets, out)
-    dev.no_autograd(gate, x, init)
+    dev.no_autograd(gate, x, init, out)
     fields, sequences, chunks = _shape(gate, x, offsets, log_gate, out is None)
+    given = out
     shape = x.shape
     state = (sequences, shape[-1])
     _state(init, *state, "init")
@@ -111,6 +112,8 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     states = dev.empty(x, chunks, torch.float32) if return_states else None
     args = capi.LinearScanArgs(*fields, *gate_args, *x_args, *out_args, dev.pointer(offsets), dev.pointer(init), final.data_ptr(), dev.pointer(states))
     _run(capi.lib().thrust_cdna4_linear_scan, args, shape[-2], device, x, "linear_scan")
+    if given is not None:
+        dev.wrote([given])
     return (out, final, states) if return_states else (out, final)
 
 
@@ -144,7 +147,7 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
     slots int32 [batch] (None: row i has slot i).  A slot outside the cache marks a padded row, whose out
     is zero.  Rows of one slot are taken in their order.  `out` may be x or gate."""
     device = dev.need_device(gate, x, state, slots, out)
-    dev.no_autograd(gate, x, state)
+    dev.no_autograd(gate, x, state, out)
     _types(gate, x)
     shape = x.shape
     if len(shape) != 2:
@@ -159,9 +162,11 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
             raise ValueError("more rows than slots")
     elif slots.dtype != torch.int32 or slots.shape != shape[:1] or not slots.is_contiguous():
         raise ValueError("slots must be int32 [batch], contiguous")
+    written = [state]
     if out is None:
         out, out_stride = dev.empty_like(x), channels
     else:
+        written.append(out)
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
@@ -176,4 +181,5 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
             rc = entry(*args)
     if rc:
         capi.check(rc, "linear_scan_step")
+    dev.wrote(written)
     return out
