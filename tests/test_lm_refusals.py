@@ -216,3 +216,55 @@ def test_an_output_that_wants_its_gradient_is_refused(any_device):
         thrust_amd.linear_scan(x, x, out=Z(1, 5, 3).requires_grad_())
     with pytest.raises(ValueError, match="differentiation"):
         thrust_amd.linear_scan_step(x[0], x[0], Z(5, 3), out=Z(5, 3).requires_grad_())
+
+
+class Handle:
+    """Stands for the tensor of a cache's pool addresses."""
+
+    def __init__(self):
+        self.recorded = []
+
+    def record_stream(self, stream):
+        self.recorded.append(stream)
+
+
+def test_what_a_call_reads_outlives_it(monkeypatch):
+    """Private memory that pending work reads is recorded on every stream but its own, once, and kept for good where a graph has it."""
+    now = {"stream": 5, "capturing": False}
+    monkeypatch.setattr(device, "stream", lambda d: now["stream"])
+    monkeypatch.setattr(device, "capturing", lambda: now["capturing"])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: now["stream"])
+    monkeypatch.setattr(device, "_CAPTURED", [])
+    on = torch.device("cuda", 0)
+    handle = Handle()
+    kept = device.Outliving(handle, on)
+    kept.used()
+    assert handle.recorded == []
+    for s, want in ((9, [9]), (9, [9]), (5, [9]), (11, [9, 11])):
+        now["stream"] = s
+        kept.used()
+        assert handle.recorded == want
+    now.update(stream=12, capturing=True)
+    kept.used()
+    kept.used()
+    assert handle.recorded == [9, 11] and device._CAPTURED == [handle]
+    now["capturing"] = False
+    kept.used()
+    assert handle.recorded == [9, 11, 12] and device._CAPTURED == [handle]
+
+
+def test_the_calls_that_copy_pages_hold_the_pools_addresses(monkeypatch):
+    class Entry:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    monkeypatch.setattr(device, "need_device", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(device, "stream", lambda d: 0)
+    monkeypatch.setattr(device, "is_current", lambda d: True)
+    monkeypatch.setattr(capi, "lib", Entry)
+    cache = thrust_amd.PageCache([Z(3, 2)], 4, 2, 2)
+    uses = []
+    monkeypatch.setattr(type(cache._pointers), "used", lambda self: uses.append(self))
+    cache.resize(Z(1).int(), Z(1).int())
+    cache.fork(Z(1).int(), Z(1).int())
+    cache.compact()
+    assert uses == [cache._pointers] * 3

@@ -561,3 +561,54 @@ def test_torch_is_told_what_is_written():
     with torch.inference_mode():  # tensors without a version
         cache, _ = make(9, POOLS["keys and values"], 4, 5, 3)
     cache.resize(ints([0, 1]), ints([5, 6]))
+
+
+@pytest.mark.needs_device
+def test_a_cache_that_is_dropped_under_a_pending_call():
+    """The addresses of its pools are in memory of its own, which no other tensor gets before the call has read it."""
+    stream, tables = torch.cuda.Stream(), []
+    for _ in range(3):
+        cache, ref = make(40, [((64,), torch.float32)] * 3, 4, 8, 5)
+        pools, rows, a, b, ids, lengths = cache.pools, cache.tables, ints([0]), ints([1]), ints([0]), ints([7])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(50_000_000)  # tens of milliseconds
+            cache.resize(ids, lengths)
+            cache.fork(a, b, share=False)
+        where = cache._pointers.tensor.data_ptr()
+        keep = [cache.lengths, cache.refs]
+        del cache
+        others = [torch.zeros(3, dtype=torch.int64, device="cuda") for _ in range(64)]
+        assert not stream.query()
+        assert all(t.data_ptr() != where for t in others)
+        torch.cuda.synchronize()
+        ref.resize([0], [7])
+        ref.fork([0], [1], False)
+        assert get(rows).tolist() == ref.tables and get(keep[0]).tolist() == ref.lengths and get(keep[1]).tolist() == ref.refs
+        assert all(torch.equal(get(p), q) for p, q in zip(pools, ref.pools))
+
+
+@pytest.mark.needs_device
+def test_a_graph_outlives_the_cache_that_it_was_captured_with():
+    cache, ref = make(40, [((64,), torch.float32)] * 3, 4, 8, 5)
+    own, ids, lengths, a, b = (cache.tables, cache.lengths, cache.refs, cache.pools), ints([0]), ints([7]), ints([0]), ints([1])
+    cache.resize(ids, lengths)
+    cache.fork(a, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.free(b)
+        done = cache.fork(a, b, share=False)
+    where = cache._pointers.tensor.data_ptr()
+    del cache
+    others = [torch.zeros(3, dtype=torch.int64, device="cuda") for _ in range(64)]
+    assert all(t.data_ptr() != where for t in others)
+    ref.resize([0], [7])
+    ref.fork([0], [1], True)
+    for r in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.free([1])
+        assert get(done).tolist() == [True] == ref.fork([0], [1], False)
+        assert get(own[0]).tolist() == ref.tables and get(own[1]).tolist() == ref.lengths and get(own[2]).tolist() == ref.refs
+        assert all(torch.equal(get(p), q) for p, q in zip(own[3], ref.pools))

@@ -47,6 +47,34 @@ def empty_like(t):
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
+def capturing():
+    return torch._C._cuda_isCurrentStreamCapturing()
+
+
+_CAPTURED = []
+
+
+class Outliving:
+    """Private memory that calls read on the device: no other tensor gets it while work on any stream may
+    still read it, also when its owner is gone.  Where a graph has captured such a call it is kept for good."""
+
+    def __init__(self, tensor, device):
+        self.tensor, self.device = tensor, device
+        self._streams, self._captured = [stream(device)], False
+
+    def used(self):
+        """Before or after a call on the current stream of the device, which is the current one."""
+        if self.device.type != "cuda":
+            return
+        if capturing():
+            if not self._captured:
+                self._captured = True
+                _CAPTURED.append(self.tensor)
+        elif (s := stream(self.device)) not in self._streams:
+            self.tensor.record_stream(torch.cuda.current_stream(self.device))
+            self._streams.append(s)
+
+
 def pointer(t):
     return None if t is None else t.data_ptr()
 

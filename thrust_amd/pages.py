@@ -41,8 +41,8 @@ class PageCache:
         self.tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
         self.lengths = self._array(lengths, (max_sequences,), 0, "lengths")
         self.refs = self._array(refs, (pages,), 0, "refs")
-        self._pointers = torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device)
-        self._args = capi.PageCacheArgs(pools=self._pointers.data_ptr(), page_bytes=total // max(pages, 1), num_pools=len(pools), num_pages=pages,
+        self._pointers = dev.Outliving(torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device), device)
+        self._args = capi.PageCacheArgs(pools=self._pointers.tensor.data_ptr(), page_bytes=total // max(pages, 1), num_pools=len(pools), num_pages=pages,
                                         page_size=page_size, num_sequences=max_sequences, max_pages=max_pages,
                                         tables=self.tables.data_ptr(), lengths=self.lengths.data_ptr(), refs=self.refs.data_ptr())
         self._ref = ctypes.byref(self._args)
@@ -66,7 +66,8 @@ class PageCache:
         return ids[0].shape[0]
 
     def _temp(self, entry, key, *args):
-        """Temporary storage for a call: asked for once, allocated each time (a graph keeps its own)."""
+        """Temporary storage for a call that copies pages: its size asked for once, allocated each time (a graph keeps its own)."""
+        self._pointers.used()
         nbytes = self._sizes.get(key)
         if nbytes is None:
             nbytes = ctypes.c_size_t(0)
