@@ -408,9 +408,10 @@ int thrust_cdna4_get_device(int* device);
 int thrust_cdna4_set_lookback_patience(int polls);
 /*
  * Test knob for that recomputation path; no counterpart in the reference.  Tile 0 of the
- * ticketless scan, scan_by_key and reduce_by_key kernels and of every pass of the sort sleeps `sleeps` times (a few
- * microseconds each, clamped to 100000) before it publishes its descriptor, so that with
- * patience 0 every later tile deterministically finds it missing, also at the second look.
+ * ticketless scan, scan_by_key and reduce_by_key kernels, of every pass of the sort and of every chain of
+ * tiles of the linear recurrence and its gradient sleeps `sleeps` times (a few microseconds each, clamped
+ * to 100000) before it publishes its descriptor, so that with patience 0 every later tile deterministically
+ * finds it missing, also at the second look.
  * Every kernel still runs to completion.  Returns the previous value; 0 (the default) switches
  * it off.
  */
@@ -451,19 +452,21 @@ int thrust_cdna4_profile_get(int index, const char** name, float* ms);
  */
 int thrust_cdna4_sort_status(const void* temp, int64_t n, void* stream);
 /*
- * Diagnostics; no counterpart in the reference.  Counts the waits that did not end (see
- * thrust_cdna4_sort_status; those of the linear recurrence among them) per device: blocks until the device is idle and stores the count
- * since the process started; anything but 0 means that some sort's result cannot be trusted.
+ * Diagnostics; no counterpart in the reference.  Counts the waits that did not end per device, those of
+ * the sort (see thrust_cdna4_sort_status), of the linear recurrence and its gradient (what was waited for
+ * then reads as NaN, and so does what follows from it) and of the template layer's kernels: blocks until the
+ * device is idle and stores the count since the process started; anything but 0 means that the result of
+ * some such call cannot be trusted.
  */
 int thrust_cdna4_lookback_timeouts(unsigned long long* count);
-/* The device address of that counter (a 32-bit unsigned word) on the current device, for kernels
- * built outside the library (the template layer's kernel templates add to it when one of their
+/* The device address of that counter (a 32-bit unsigned word, the only one) on the current device, for
+ * kernels built outside the library (the template layer's kernel templates add to it when one of their
  * own bounded waits gives up). */
 int thrust_cdna4_lookback_timeout_counter(void** device_address);
 /*
  * Test knob for that error path; no counterpart in the reference.  The number of polls after
- * which a wait inside the sort gives up (negative: the default, about 4 million); returns the
- * previous value.  With 0 and thrust_cdna4_set_test_publish_delay, tile 0 of a pass publishes
+ * which a wait inside the sort, the linear recurrence or its gradient gives up (negative: the default, about 4
+ * million); returns the previous value.  With 0 and thrust_cdna4_set_test_publish_delay, tile 0 of a pass publishes
  * late, the tiles that look for it give up at once, every kernel still runs to completion, and
  * thrust_cdna4_sort_status reports the time-out.
  */

@@ -14,3 +14,8 @@ def test_nothing_outside_the_ranges(emulated_library):  # noqa: F811
 def test_tiles_in_flight(emulated_library, resident):  # noqa: F811
     print(run_session(["tests/test_linear_scan_gpu.py", "tests/test_pages_gpu.py"], resident=resident,
                       extra=["-k", "many_tiles or past_super or packed or vary or fork or resize or compact or life"]))
+
+
+@pytest.mark.parametrize("resident", ["1", "40:9"])
+def test_waits_that_are_given_up(emulated_library, resident):  # noqa: F811
+    print(run_session(["tests/test_zw_recurrence_timeout_gpu.py"], resident=resident))

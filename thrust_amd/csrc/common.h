@@ -429,8 +429,10 @@ __global__ void zero_words_kernel(uint32_t* p, size_t nwords);
 // of 8 would fault on the device, so such a call is refused on the host (the interface asks for 256).
 inline bool temp_misaligned(const void* temp) { return (reinterpret_cast<uintptr_t>(temp) & 7u) != 0; }
 
-// waits of the linear recurrence that did not end, on the current device (linear_scan.hip)
-hipError_t linear_scan_timeouts(unsigned int* count);
+// Where kernels of other files count their waits that did not end: the word of thrust_cdna4_lookback_timeouts
+// on the current device, and the polls after which a wait gives up (sort.hip).
+hipError_t lookback_timeout_counter(uint32_t** address);
+uint32_t lookback_spin_limit();
 
 hipError_t zero_async(void* p, size_t bytes, hipStream_t stream);
 // dst[0, bytes) = src[0, bytes) on the device, enqueued on `stream` (non-overlapping ranges)

@@ -53,9 +53,6 @@ constexpr int kLinTicketWords = 32;
 constexpr int kLinSuper = kLinGroup * kLinGroup;
 constexpr int kLinChunk = THRUST_CDNA4_LINEAR_SCAN_CHUNK;
 constexpr int64_t kLinMaxChannels = int64_t(1) << 28;  // a lane's offset in a row of maps is 32 bits of bytes
-constexpr uint32_t kLinSpinLimit = 1u << 22;  // polls; seconds
-
-__device__ unsigned int g_linear_scan_timeouts;
 
 struct LinArgs {
   const void* gate;
@@ -76,6 +73,9 @@ struct LinArgs {
   uint64_t* tile_map;   // [batch][ntiles][channels]
   uint64_t* group_map;  // [batch][groups][channels]
   uint32_t* super_state;  // [batch][super-groups][channels]
+  uint32_t* timeouts;     // waits that were given up
+  uint32_t spin_limit;    // polls after which they are; seconds
+  int publish_delay;
 };
 
 // ---------------------------------------------------------------------------------------
@@ -290,7 +290,7 @@ __device__ inline float group_state(const LinShared<CH>& sm, int ch) {
 
 // Waits until n words that start `stride` elements apart are published; they have been asked for once.
 template <int N, class W>
-__device__ inline void wait_words(const W* p, int64_t stride, uint32_t c, W (&v)[N]) {
+__device__ inline void wait_words(const LinArgs& args, const W* p, int64_t stride, uint32_t c, W (&v)[N]) {
   // The ticket order makes every predecessor a running workgroup, so these waits end; the limit keeps a
   // mistake from hanging the device, and is counted (thrust_cdna4_lookback_timeouts); what was waited for
   // then reads as NaN.
@@ -299,13 +299,13 @@ __device__ inline void wait_words(const W* p, int64_t stride, uint32_t c, W (&v)
 #pragma unroll
     for (int k = 0; k < N; k++) all = all && v[k] != 0;
     if (all) return;
-    if (spins >= kLinSpinLimit) break;
+    if (spins >= args.spin_limit) break;
     __builtin_amdgcn_s_sleep(1);
 #pragma unroll
     for (int k = 0; k < N; k++)
       if (v[k] == 0) v[k] = ld_agent(at(p + k * stride, c));
   }
-  atomicAdd(&g_linear_scan_timeouts, 1u);
+  atomicAdd(args.timeouts, 1u);
 }
 
 // Called by the whole workgroup after sm.m, sm.e, sm.h, sm.anew and sm.since are written and a barrier.
@@ -341,6 +341,8 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
   };
   const Product one{1.f, 0};
   if (role == 0 && from < C) {
+    if (i == 0)
+      for (int k = 0; k < p.publish_delay; k++) __builtin_amdgcn_s_sleep(127);  // test knob, 0 in normal use
     if (publishes) publish_map(at(p.tile_map + ((int64_t)b * nt + i) * C, chan), tile_after(one, 0.f));
     __builtin_amdgcn_sched_barrier(0);  // the folded maps' registers are free for the words that follow
     const uint64_t* maps = p.tile_map + ((int64_t)b * nt + base) * C;
@@ -348,7 +350,7 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
     uint64_t v[N];
 #pragma unroll
     for (int k = 0; k < N; k++) v[k] = k >= k0 && k < k1 ? ld_agent(at(maps + k * C, chan)) : ~uint64_t(0);
-    wait_words(maps, C, chan, v);
+    wait_words(p, maps, C, chan, v);
     // (GA, GH): the map of the group's earlier tiles, or GH a state where the sequence begins among them
     Product GA = one;
     float GH = 0.f;
@@ -379,8 +381,8 @@ __device__ inline void tile_carry(LinShared<kWave * VEC>& sm, const LinArgs& p, 
 #pragma unroll
       for (int k = 0; k < N; k++) v[k] = k >= k0 && k < k1 ? ld_agent(at(maps + k * C, chan)) : ~uint64_t(0);
       if (from_super) state[0] = ld_agent(at(states, chan));
-      wait_words(maps, C, chan, v);
-      wait_words(states, 0, chan, state);
+      wait_words(p, maps, C, chan, v);
+      wait_words(p, states, 0, chan, state);
       H = bit_cast<float>(~state[0]);
 #pragma unroll
       for (int k = 0; k < N; k++) {
@@ -904,7 +906,7 @@ inline bool lin_plan(int64_t batch, int64_t rows, int64_t channels, int tile_row
   return true;
 }
 
-inline void lin_storage(LinArgs& p, const LinPlan& l, void* temp) {
+inline hipError_t lin_storage(LinArgs& p, const LinPlan& l, void* temp) {
   p.ntiles = (int)l.ntiles;
   p.ncb = l.ncb;
   p.tickets = nullptr;
@@ -914,7 +916,11 @@ inline void lin_storage(LinArgs& p, const LinPlan& l, void* temp) {
     p.tile_map = reinterpret_cast<uint64_t*>(t + l.tile_at);
     p.group_map = reinterpret_cast<uint64_t*>(t + l.group_at);
     p.super_state = reinterpret_cast<uint32_t*>(t + l.super_at);
+    p.spin_limit = lookback_spin_limit();
+    p.publish_delay = lookback_test_publish_delay();
+    return lookback_timeout_counter(&p.timeouts);
   }
+  return hipSuccess;
 }
 
 // rows of the recurrence's tile: the payload of a lane is 64 registers at most
@@ -983,7 +989,8 @@ extern "C" int thrust_cdna4_linear_scan(void* temp, size_t* temp_bytes, const th
     p.x_bs = a->x_batch_stride, p.x_rs = a->x_row_stride;
     p.out_bs = a->out_batch_stride, p.out_rs = a->out_row_stride;
     p.rows = a->rows, p.channels = a->channels, p.batch = (int)a->batch, p.log_gate = a->log_gate != 0, p.clear_outside = packed && a->clear_outside;
-    lin_storage(p, l, temp);
+    rc = lin_storage(p, l, temp);
+    if (rc != hipSuccess) return;
     if (l.clear) {
       rc = zero_async(temp, l.clear, s);
       if (rc != hipSuccess) return;
@@ -1051,7 +1058,8 @@ extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes,
     p.grad_bs = a->grad_out_batch_stride, p.grad_rs = a->grad_out_row_stride;
     p.grad_gate_bs = a->grad_gate_batch_stride, p.grad_gate_rs = a->grad_gate_row_stride;
     p.rows = a->rows, p.channels = a->channels, p.batch = (int)a->batch, p.log_gate = a->log_gate != 0, p.clear_outside = packed && a->clear_outside;
-    lin_storage(p, l, temp);
+    rc = lin_storage(p, l, temp);
+    if (rc != hipSuccess) return;
     if (l.clear) {
       rc = zero_async(temp, l.clear, s);
       if (rc != hipSuccess) return;
@@ -1112,10 +1120,3 @@ extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int lo
   });
   return (int)rc;
 }
-
-namespace tcd {
-// waits of this file's kernels that did not end, on the current device
-hipError_t linear_scan_timeouts(unsigned int* count) {
-  return hipMemcpyFromSymbol(count, HIP_SYMBOL(g_linear_scan_timeouts), sizeof(*count));
-}
-}  // namespace tcd

@@ -898,6 +898,20 @@ __global__ __launch_bounds__(kFillThreads) void counting_fill_kernel(uint8_t* ou
 constexpr int kHistDoneWord = 8;  // in the 64 words of the ticket block
 constexpr size_t kSortStatusOffset = 0;  // of the status word in a sort call's temporary storage
 static std::atomic<uint32_t> g_test_spin_limit{kLookbackSpinLimit};  // test knob
+uint32_t lookback_spin_limit() { return g_test_spin_limit.load(std::memory_order_relaxed); }
+hipError_t lookback_timeout_counter(uint32_t** address) {
+  static std::atomic<uint32_t*> cached[kMaxDevices];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const bool known = dev >= 0 && dev < kMaxDevices;
+  if (known && (*address = cached[dev].load(std::memory_order_relaxed))) return hipSuccess;
+  void* p = nullptr;
+  e = hipGetSymbolAddress(&p, HIP_SYMBOL(g_lookback_timeouts));
+  *address = static_cast<uint32_t*>(p);
+  if (e == hipSuccess && known) cached[dev].store(*address, std::memory_order_relaxed);
+  return e;
+}
 static constexpr size_t xcd_words_per_pass(int slots) { return (size_t)kXcds * kXcdCounterStride + (size_t)kXcds * (size_t)slots; }
 template <class U, int VB, class C, class D>
 static SortPlan make_plan(int64_t n) {
@@ -952,7 +966,7 @@ static hipError_t sort_with(void* temp, size_t* temp_bytes, void* keys, void* va
   D* desc = reinterpret_cast<D*>(t + plan.desc);
   static_assert(kSortStatusOffset == 0, "thrust_cdna4_sort_status reads the first word");
   uint32_t* status = reinterpret_cast<uint32_t*>(t + plan.status);
-  const uint32_t spin_limit = g_test_spin_limit.load(std::memory_order_relaxed);
+  const uint32_t spin_limit = lookback_spin_limit();
   const int publish_delay = lookback_test_publish_delay();
 
   hipError_t e = zero_async(t + plan.zero_begin, plan.zero_bytes, stream);
@@ -1119,10 +1133,9 @@ extern "C" int thrust_cdna4_lookback_timeout_counter(void** device_address) {
 
 extern "C" int thrust_cdna4_lookback_timeouts(unsigned long long* count) {
   if (!count) return hipErrorInvalidValue;
-  unsigned int c = 0, linear = 0;
-  hipError_t e = hipMemcpyFromSymbol(&c, HIP_SYMBOL(tcd::g_lookback_timeouts), sizeof(c));
-  if (e == hipSuccess) e = tcd::linear_scan_timeouts(&linear);
-  *count = (unsigned long long)c + linear;
+  unsigned int c = 0;
+  const hipError_t e = hipMemcpyFromSymbol(&c, HIP_SYMBOL(tcd::g_lookback_timeouts), sizeof(c));
+  *count = c;
   return (int)e;
 }
 
