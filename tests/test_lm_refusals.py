@@ -268,3 +268,68 @@ def test_the_calls_that_copy_pages_hold_the_pools_addresses(monkeypatch):
     cache.fork(Z(1).int(), Z(1).int())
     cache.compact()
     assert uses == [cache._pointers] * 3
+
+
+# `out` may be x or gate; every other overlap of an output with an input would be written while it is read
+OVERLAPS = {  # of a buffer [9, 2, 12]
+    "shifted by a row": lambda b: (b[1:7, 0, :4][None], b[0:6, 0, :4][None]),
+    "shifted by a column": lambda b: (b[0:6, 0, 1:5][None], b[0:6, 0, 0:4][None]),
+    "at another pitch": lambda b: (b.flatten()[:24].view(1, 6, 4), b.flatten()[8:80].view(1, 6, 12)[..., :4]),
+    "batches for rows": lambda b: (b[0:2, :, :4], b.as_strided((2, 2, 4), (12, 24, 1))),
+    "a row of it": lambda b: (b[0:6, 0, :4][None], b[3:4, 0, :4].expand(6, 4)[None]),
+}
+
+
+@pytest.mark.parametrize("which", list(OVERLAPS), ids=str)
+def test_an_output_that_meets_an_input_is_refused(any_device, which):
+    out, other = OVERLAPS[which](Z(9, 2, 12))
+    fresh = torch.zeros(out.shape)
+    for gate, x in ((other, fresh), (fresh, other)):
+        with pytest.raises(ValueError, match="shares memory"):
+            thrust_amd.linear_scan(gate, x, out=out)
+        if len(out) == 1:
+            with pytest.raises(ValueError, match="shares memory"):
+                thrust_amd.linear_scan_step(gate[0], x[0], Z(8, 4), out=out[0])
+    state = Z(8, 4)
+    with pytest.raises(ValueError, match="shares memory"):
+        thrust_amd.linear_scan_step(fresh[0], fresh[0], state, out=state[1:1 + fresh.shape[1]])
+    with pytest.raises(ValueError, match="shares memory"):
+        thrust_amd.linear_scan_step(state[2:2 + fresh.shape[1]], fresh[0], state)
+    rows = Z(3, 4)
+    with pytest.raises(ValueError, match="shares memory"):
+        thrust_amd.linear_scan(Z(1, 3, 4), Z(1, 3, 4), init=rows[1:2], out=rows[None])
+
+
+def test_whether_views_share_an_element():
+    """Against the sets of addresses, over random views of one buffer."""
+    from thrust_amd import recurrence
+    g = torch.Generator().manual_seed(2)
+
+    def pick(low, high):
+        return int(torch.randint(low, high + 1, (1,), generator=g))
+
+    def addresses(t):
+        at = [t.data_ptr()]
+        for n, s in zip(t.shape, t.stride()):
+            at = [a + k * s * t.element_size() for a in at for k in range(n)]
+        return {a + k for a in at for k in range(t.element_size())}
+    met = 0
+    for _ in range(3000):
+        buffer = torch.zeros(400)
+        views = []
+        for _ in range(2):
+            c, n, b = pick(1, 5), pick(1, 5), pick(1, 3)
+            rs = pick(0 if views else c, 12)
+            bs = pick(0, 40) if views else rs * n + pick(0, 8)
+            if views and pick(0, 1):
+                (c, n, b), (bs, rs) = views[0].shape[::-1], views[0].stride()[:2]
+            v = buffer if pick(0, 3) else buffer.view(torch.bfloat16)
+            views.append(v.as_strided((b, n, c), (bs, rs, 1), pick(0, 150)))
+        out, t = views
+        want = bool(addresses(out) & addresses(t))
+        met += want
+        assert recurrence._meet(out, t) == want, (out.shape, out.stride(), out.storage_offset(), t.shape, t.stride(), t.storage_offset())
+    assert 500 < met < 2500
+    assert not recurrence._meet(torch.zeros(0, 3), buffer) and not recurrence._meet(buffer[:0].view(0, 2, 3), buffer)
+    big = torch.zeros(1, 8).expand(1 << 40, 8)  # a row that is read again and again is one
+    assert recurrence._meet(big[:1, :3], big)

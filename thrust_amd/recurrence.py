@@ -40,6 +40,49 @@ def _distinct(t, what):
         need = stride * (size - 1) + need
 
 
+def _span(t):
+    """Bytes from the first element to behind the last one."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _rows_at(t):
+    """The addresses at which the rows of t begin, ascending, and the bytes of one."""
+    at = torch.tensor([t.data_ptr()])
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        if n > 1 and s > 0:
+            at = (at[:, None] + torch.arange(n) * (s * t.element_size())).flatten()
+    return at.sort().values, t.shape[-1] * t.element_size()
+
+
+def _layout(t):
+    return [s * t.element_size() for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+
+
+def _meet(a, b):
+    """Whether two tensors share memory.  (Channels are next to each other in both.)"""
+    if not a.numel() or not b.numel() or a.data_ptr() >= b.data_ptr() + _span(b) or b.data_ptr() >= a.data_ptr() + _span(a):
+        return False
+    pitches, row = _layout(a), a.shape[-1] * a.element_size()
+    if pitches and a.shape == b.shape and pitches == _layout(b) and min(pitches) > 0 and not any(s % min(pitches) for s in pitches):
+        apart = (a.data_ptr() - b.data_ptr()) % min(pitches)  # columns of one array, as the parts of one projection are
+        if apart >= b.shape[-1] * b.element_size() and min(pitches) - apart >= row:
+            return False
+    (rows_a, row_a), (rows_b, row_b) = _rows_at(a), _rows_at(b)
+    return bool((torch.searchsorted(rows_a, rows_b + row_b) > torch.searchsorted(rows_a, rows_b - row_a, right=True)).any())
+
+
+def _apart(out, tensors, inputs=()):
+    """Refuses an output that shares memory with one of `tensors`, or of `inputs` without being it."""
+    for t in inputs:
+        if t.data_ptr() == out.data_ptr() and t.dtype == out.dtype and _layout(t) == _layout(out):
+            continue
+        if _meet(out, t):
+            raise ValueError("an output shares memory with an input, and is not the same tensor")
+    for t in tensors:
+        if t is not None and _meet(out, t):
+            raise ValueError("an output shares memory with an input")
+
+
 def _state(t, sequences, channels, what):
     if t is None:
         return
@@ -91,7 +134,7 @@ def _run(entry, args, rows, device, x, what):
 def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, return_states=False):
     """h[t] = a[t] * h[t-1] + x[t]; returns (out, final): every h in the type of x, and the last one of
     each sequence in float32.  `init`: the states before the first rows (zero if None).  `out` may be x
-    or gate.  return_states: also the state that enters each chunk of 64 rows, for linear_scan_backward.
+    or gate; one that shares memory with them, or with init, in another way is refused.  return_states: also the state that enters each chunk of 64 rows, for linear_scan_backward.
     Packed rows that belong to no sequence are left as they were in a given `out`, and zero in a new one."""
     device = dev.need_device(gate, x, init, offsets, out)
     dev.no_autograd(gate, x, init, out)
@@ -107,6 +150,8 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
+        _rows(out, shape, "out")
+        _apart(out, (init, offsets), (gate, x))
     out_args = _strided(out, shape, "out")
     final = dev.empty(x, state, torch.float32) if init is None else dev.empty_like(init)
     states = dev.empty(x, chunks, torch.float32) if return_states else None
@@ -145,7 +190,8 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
     """One row for each of a batch: state[slots[i]] = a[i] * state[slots[i]] + x[i], in place; returns the
     new states in the type of x.  gate and x are [batch, channels], state float32 [slots, channels],
     slots int32 [batch] (None: row i has slot i).  A slot outside the cache marks a padded row, whose out
-    is zero.  Rows of one slot are taken in their order.  `out` may be x or gate."""
+    is zero.  Rows of one slot are taken in their order.  `out` may be x or gate;
+    otherwise out and state share no memory with each other and the inputs."""
     device = dev.need_device(gate, x, state, slots, out)
     dev.no_autograd(gate, x, state, out)
     _types(gate, x)
@@ -171,8 +217,13 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
         out_stride = _rows(out, shape, "out")[1]
-    args = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate.data_ptr(), _rows(gate, shape, "gate")[1], x.data_ptr(), _rows(x, shape, "x")[1],
-            out.data_ptr(), out_stride, state.data_ptr(), num_slots, dev.pointer(slots), batch, channels, dev.stream(device))
+        _apart(out, (state, slots), (gate, x))
+    gate_stride, x_stride, gate_at, x_at, state_at = _rows(gate, shape, "gate")[1], _rows(x, shape, "x")[1], gate.data_ptr(), x.data_ptr(), state.data_ptr()
+    behind = state_at + num_slots * channels * 4
+    if (gate_at < behind and state_at < gate_at + (batch * gate_stride + channels) * 4) or (x_at < behind and state_at < x_at + (batch * x_stride + channels) * 4):
+        _apart(state, (gate, x))  # asked again, exactly
+    args = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate_at, gate_stride, x_at, x_stride,
+            out.data_ptr(), out_stride, state_at, num_slots, dev.pointer(slots), batch, channels, dev.stream(device))
     entry = capi.lib().thrust_cdna4_linear_scan_step
     if dev.is_current(device):
         rc = entry(*args)
