@@ -333,3 +333,13 @@ def test_whether_views_share_an_element():
     assert not recurrence._meet(torch.zeros(0, 3), buffer) and not recurrence._meet(buffer[:0].view(0, 2, 3), buffer)
     big = torch.zeros(1, 8).expand(1 << 40, 8)  # a row that is read again and again is one
     assert recurrence._meet(big[:1, :3], big)
+
+
+@pytest.mark.parametrize("what", ["tables", "lengths", "refs"])
+def test_a_caches_arrays_are_not_replaced(any_device, what):
+    """The calls go on with the arrays that the cache was made with: another one in their place would be passed over."""
+    cache = thrust_amd.PageCache([Z(3, 2)], 4, 2, 2)
+    was = getattr(cache, what)
+    with pytest.raises(AttributeError):
+        setattr(cache, what, was.clone())
+    assert getattr(cache, what) is was

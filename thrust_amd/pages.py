@@ -20,8 +20,13 @@ class PageCache:
     lengths int32 [max_sequences]             tokens; the first ceil(length / page_size) entries are held
     refs    int32 [pages]                     how many tables name a page
 
-    They start empty, or are the given ones, which are then used in place.
+    They start empty, or are the given ones, which are then used in place; their contents may be written
+    between calls, but they are not replaced by others (make a cache with those instead).
     """
+
+    tables = property(lambda self: self._tables)
+    lengths = property(lambda self: self._lengths)
+    refs = property(lambda self: self._refs)
 
     def __init__(self, pools, page_size, max_sequences, max_pages, tables=None, lengths=None, refs=None):
         pools = list(pools)
@@ -38,9 +43,9 @@ class PageCache:
         if page_size < 1 or max_sequences < 0 or max_pages < 0 or page_size * max_pages > 0x7fffffff:
             raise ValueError("page_size must be positive, and page_size * max_pages below 2^31")
         self.pools, self.page_size, self.device = pools, page_size, device
-        self.tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
-        self.lengths = self._array(lengths, (max_sequences,), 0, "lengths")
-        self.refs = self._array(refs, (pages,), 0, "refs")
+        self._tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
+        self._lengths = self._array(lengths, (max_sequences,), 0, "lengths")
+        self._refs = self._array(refs, (pages,), 0, "refs")
         self._pointers = dev.Outliving(torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device), device)
         self._args = capi.PageCacheArgs(pools=self._pointers.tensor.data_ptr(), page_bytes=total // max(pages, 1), num_pools=len(pools), num_pages=pages,
                                         page_size=page_size, num_sequences=max_sequences, max_pages=max_pages,
