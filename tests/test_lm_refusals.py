@@ -343,3 +343,11 @@ def test_a_caches_arrays_are_not_replaced(any_device, what):
     with pytest.raises(AttributeError):
         setattr(cache, what, was.clone())
     assert getattr(cache, what) is was
+
+
+def test_compact_refuses_outputs_that_meet_the_caches_arrays(any_device):
+    rows, counts = torch.full((5, 2), -1, dtype=torch.int32), Z(9).int()
+    cache = thrust_amd.PageCache([Z(3, 2)], 4, 4, 2, tables=rows[:4], refs=counts[:3])
+    for tables, refs in ((rows[1:], Z(3).int()), (Z(4, 2).int(), counts[2:5]), (Z(4, 2).int(), rows.flatten()[:3])):
+        with pytest.raises(ValueError, match="share memory"):
+            cache.compact(tables=tables, refs=refs)

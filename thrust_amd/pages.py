@@ -11,6 +11,11 @@ import torch
 from . import capi, device as dev
 
 
+def _overlap(a, b):
+    """Whether two contiguous tensors of 32 bits share memory."""
+    return a.numel() and b.numel() and a.data_ptr() < b.data_ptr() + 4 * b.numel() and b.data_ptr() < a.data_ptr() + 4 * a.numel()
+
+
 class PageCache:
     """`pools`: the arrays that are paged together (a layer's keys, its values, its recurrent states ...),
     each [pages, ...], contiguous, of any type, with the same number of pages and of bytes a page.  A page
@@ -129,6 +134,10 @@ class PageCache:
             raise ValueError("tensors on another device than the cache")
         tables = self.tables if tables is None else self._array(tables, self.tables.shape, None, "tables")
         refs = self.refs if refs is None else self._array(refs, self.refs.shape, None, "refs")
+        for new, own in ((tables, self.tables), (refs, self.refs)):
+            for t in self._own:
+                if not (t is own and new.data_ptr() == own.data_ptr()) and _overlap(new, t):
+                    raise ValueError("the outputs share memory with the cache's arrays, and are not the same")
         L = capi.lib()
         live = dev.empty(self.refs, (1,), torch.int32)
         with dev.current(self.device):
