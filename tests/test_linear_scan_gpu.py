@@ -6,6 +6,7 @@ import torch
 
 import gpu_util
 import thrust_amd
+from conftest import EMULATED
 from lm_util import Recurrence, check, get, put
 from thrust_amd import capi
 
@@ -580,3 +581,35 @@ def test_torch_is_told_what_is_written():
     assert rows._version == was[0] and state._version > was[1] and out._version > was[2]
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+# batches that are large enough for four vectors a thread: two workgroups to each of 256 compute units, or of the emulator's 8
+WIDE = [(20, c) if EMULATED else (b, c) for b, c in ((600, 1030), (600, 2051), (520, 4096), (300, 4101), (270, 8190))]
+
+
+@pytest.mark.parametrize("gate_t,x_t", [(F32, F32), (F16, F16), (F32, BF16)], ids=name)
+@pytest.mark.parametrize("batch,channels", WIDE, ids=str)
+def test_step_of_a_large_batch_of_wide_rows(batch, channels, gate_t, x_t):
+    """Every vector of a thread, the partial one behind the last whole one, several blocks of channels; rows of one slot and padded ones."""
+    log = channels % 2 == 0
+    gate, x, _, _, _ = inputs(70 + batch, (batch, channels), batch, gate_t, x_t, log)
+    g = torch.Generator().manual_seed(channels)
+    state = torch.randn((batch + 5, channels), generator=g)
+    slots = torch.randperm(batch + 5, generator=g)[:batch].int()
+    slots[3], slots[7], slots[11], slots[batch - 1] = -1, slots[1], slots[1], slots[0]
+    want, after, error, error_state = step_reference(gate, x, state, slots.tolist(), log)
+    wide = put(torch.full((batch, 2 * channels + 3), 7.0).to(x_t))
+    for rows in ("apart", "halves of a projection"):
+        on, a, b = put(state), put(gate), put(x)
+        if rows != "apart" and gate_t == x_t:
+            both = put(torch.cat([gate, x], -1))
+            a, b = both[:, :channels], both[:, channels:]
+        out = None if rows == "apart" else wide[:, channels + 1:-2]
+        got = thrust_amd.linear_scan_step(a, b, on, slots=put(slots), log_gate=log, out=out)
+        check(get(got), want, error, "out")
+        check(get(on), after, error_state, "state")
+    assert (get(wide)[:, : channels + 1] == 7).all() and (get(wide)[:, -2:] == 7).all()
+    on = put(state)
+    assert thrust_amd.linear_scan_step(a, b, on, slots=put(slots), log_gate=log, out=b) is b  # in place
+    check(get(b), want, error, "in place")
+    check(get(on), after, error_state, "state")
