@@ -34,3 +34,7 @@ def test_no_data_race_between_wavefronts(resident):
     p = subprocess.run([os.path.join(EMU_DIR, "build", "tsan", "race_lm")], env=env, capture_output=True, text=True, timeout=900)
     out = p.stdout + p.stderr
     assert p.returncode == 0 and "race_lm: done" in out and "ThreadSanitizer" not in out, out[-4000:]
+
+
+def test_the_measured_cases_at_small_sizes(emulated_library):  # noqa: F811
+    print(run_session(["tests/test_lm_cases_gpu.py"], resident="5:8"))
