@@ -262,7 +262,7 @@ int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes, const thru
  * [num_slots][channels], contiguous, updated in place; `slots` a DEVICE array.  A row whose slot is
  * negative or not below num_slots is padding: its out is zero and no state changes.  Rows of one slot
  * are successive tokens of one sequence and taken in their order.  Needs no temporary storage.  The
- * arrays must not overlap, except that out may be x or gate itself.
+ * arrays must not overlap, except that out may be x or gate itself; a state that meets gate, x or out is refused.
  */
 int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, const void* gate, int64_t gate_row_stride,
                                   const void* x, int64_t x_row_stride, void* out, int64_t out_row_stride, void* state,
@@ -320,7 +320,8 @@ int thrust_cdna4_pages_free(const thrust_cdna4_page_cache* cache, const int32_t*
 /*
  * Moves pages until those in use are the lowest: the highest page in use moves to the lowest free one,
  * and so on.  Writes the renumbered tables and refs to tables_out and refs_out, which may be those
- * of the cache, and the number of pages in use to live_out (DEVICE, int32).  The pages moved from keep
+ * of the cache (and otherwise must not meet its arrays or each other, which is refused), and the number of
+ * pages in use to live_out (DEVICE, int32).  The pages moved from keep
  * their contents: work in flight with the old tables may end.
  */
 int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const thrust_cdna4_page_cache* cache, int32_t* tables_out,

@@ -613,3 +613,20 @@ def test_step_of_a_large_batch_of_wide_rows(batch, channels, gate_t, x_t):
     assert thrust_amd.linear_scan_step(a, b, on, slots=put(slots), log_gate=log, out=b) is b  # in place
     check(get(b), want, error, "in place")
     check(get(on), after, error_state, "state")
+
+
+def test_a_state_between_the_rows_of_an_input():
+    """Ranges that meet without an element in common are no overlap."""
+    gate, x, _, _, _ = inputs(80, (3, 4), 3, F32, F32, False)
+    init = torch.randn((2, 4), generator=torch.Generator().manual_seed(1))
+    buffer = torch.zeros(3, 12)
+    buffer[:, :4] = x
+    buffer[1, 4:] = init.flatten()
+    on = put(buffer)
+    state = on.flatten()[16:24].view(2, 4)
+    slots = torch.tensor([1, 0, 1], dtype=torch.int32)
+    out = thrust_amd.linear_scan_step(put(gate), on[:, :4], state, slots=put(slots))
+    want, after, error, error_state = step_reference(gate, x, init, slots.tolist(), False)
+    check(get(out), want, error, "out")
+    check(get(state), after, error_state, "state")
+    assert torch.equal(get(on)[:, :4], x)

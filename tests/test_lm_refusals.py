@@ -1,5 +1,6 @@
 """CPU-only: what the entry points of the linear recurrence and the page cache refuse, and their size
 queries, which touch no device."""
+import contextlib
 import ctypes
 
 import pytest
@@ -236,21 +237,23 @@ def test_what_a_call_reads_outlives_it(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: now["stream"])
     monkeypatch.setattr(device, "_CAPTURED", [])
     on = torch.device("cuda", 0)
-    handle = Handle()
-    kept = device.Outliving(handle, on)
-    kept.used()
-    assert handle.recorded == []
-    for s, want in ((9, [9]), (9, [9]), (5, [9]), (11, [9, 11])):
-        now["stream"] = s
-        kept.used()
-        assert handle.recorded == want
-    now.update(stream=12, capturing=True)
-    kept.used()
-    kept.used()
-    assert handle.recorded == [9, 11] and device._CAPTURED == [handle]
-    now["capturing"] = False
-    kept.used()
-    assert handle.recorded == [9, 11, 12] and device._CAPTURED == [handle]
+    for own in (5, 0):
+        now.update(stream=own, capturing=False)
+        handle = Handle()
+        kept = device.Outliving(handle, on)
+        kept.used(own)
+        assert handle.recorded == []
+        for s, want in ((9, [9]), (9, [9]), (own, [9]), (11, [9, 11])):
+            now["stream"] = s
+            kept.used(s)
+            assert handle.recorded == want
+        now.update(stream=12, capturing=True)
+        kept.used(12)
+        kept.used(12)
+        assert handle.recorded == [9, 11] and device._CAPTURED[-1] is handle and device._CAPTURED.count(handle) == 1
+        now["capturing"] = False
+        kept.used(12)
+        assert handle.recorded == [9, 11, 12]
 
 
 def test_the_calls_that_copy_pages_hold_the_pools_addresses(monkeypatch):
@@ -261,13 +264,17 @@ def test_the_calls_that_copy_pages_hold_the_pools_addresses(monkeypatch):
     monkeypatch.setattr(device, "stream", lambda d: 0)
     monkeypatch.setattr(device, "is_current", lambda d: True)
     monkeypatch.setattr(capi, "lib", Entry)
+    monkeypatch.setattr(device, "stream", lambda d: 3)
     cache = thrust_amd.PageCache([Z(3, 2)], 4, 2, 2)
     uses = []
-    monkeypatch.setattr(type(cache._pointers), "used", lambda self: uses.append(self))
+    monkeypatch.setattr(type(cache._pointers), "used", lambda self, stream: uses.append(self))
     cache.resize(Z(1).int(), Z(1).int())
     cache.fork(Z(1).int(), Z(1).int())
     cache.compact()
     assert uses == [cache._pointers] * 3
+    monkeypatch.setattr(device, "stream", lambda d: 0)  # back on the default one, which is not where it was made
+    cache.compact()
+    assert uses == [cache._pointers] * 4
 
 
 # `out` may be x or gate; every other overlap of an output with an input would be written while it is read
@@ -293,11 +300,25 @@ def test_an_output_that_meets_an_input_is_refused(any_device, which):
     state = Z(8, 4)
     with pytest.raises(ValueError, match="shares memory"):
         thrust_amd.linear_scan_step(fresh[0], fresh[0], state, out=state[1:1 + fresh.shape[1]])
-    with pytest.raises(ValueError, match="shares memory"):
-        thrust_amd.linear_scan_step(state[2:2 + fresh.shape[1]], fresh[0], state)
     rows = Z(3, 4)
     with pytest.raises(ValueError, match="shares memory"):
         thrust_amd.linear_scan(Z(1, 3, 4), Z(1, 3, 4), init=rows[1:2], out=rows[None])
+
+
+def test_a_state_that_meets_what_a_step_reads_or_writes_is_refused(any_device, monkeypatch):
+    monkeypatch.setattr(device, "is_current", lambda d: True)  # it is the entry point that refuses, before anything is launched
+    rows = Z(8, 12)
+    state, x = rows.flatten()[:32].view(8, 4), Z(3, 4)
+    for other in (state[2:5], rows[2:5, 4:8], rows[0:1, 8:].expand(3, 4), rows.view(torch.int32).view(torch.float32)[1:4, :4]):
+        for gate, v in ((other, x), (x, other)):
+            with pytest.raises(ValueError, match="shares memory"):
+                thrust_amd.linear_scan_step(gate, v, state)
+    call = capi.lib().thrust_cdna4_linear_scan_step
+
+    def meets(at, pitch, batch=5, channels=4, slots=8, state=0x100000):
+        return call(capi.F32, capi.F32, 0, 0x1000, 4, at, pitch, 0x4000, 4, state, slots, None, batch, channels, None)
+    for at, pitch in ((0x100000, 4), (0x100000 - 16 * 4, 4), (0x100000 - 15, 0), (0x100000 - 4 * 4 * 1000 - 15, 1000), (0x100000 + 127, 1000)):
+        assert meets(at, pitch) == INVALID, (hex(at), pitch)
 
 
 def test_whether_views_share_an_element():
@@ -345,7 +366,8 @@ def test_a_caches_arrays_are_not_replaced(any_device, what):
     assert getattr(cache, what) is was
 
 
-def test_compact_refuses_outputs_that_meet_the_caches_arrays(any_device):
+def test_compact_refuses_outputs_that_meet_the_caches_arrays(any_device, monkeypatch):
+    monkeypatch.setattr(device, "current", lambda d: contextlib.nullcontext())  # it is the entry point that refuses, before anything is launched
     rows, counts = torch.full((5, 2), -1, dtype=torch.int32), Z(9).int()
     cache = thrust_amd.PageCache([Z(3, 2)], 4, 4, 2, tables=rows[:4], refs=counts[:3])
     for tables, refs in ((rows[1:], Z(3).int()), (Z(4, 2).int(), counts[2:5]), (Z(4, 2).int(), rows.flatten()[:3])):

@@ -939,6 +939,16 @@ inline size_t span_bytes(int64_t batch, int64_t rows, int64_t channels, int64_t 
   return (size_t)((batch - 1) * bs + (rows - 1) * rs + channels) * (size_t)elem;
 }
 
+// whether rows of `row` bytes, `pitch` >= 0 apart, meet [b, b + nb)
+inline bool rows_meet(const void* a, int64_t rows, int64_t pitch, size_t row, const void* b, size_t nb) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(a), lo = reinterpret_cast<uintptr_t>(b);
+  if (rows <= 0 || row == 0 || nb == 0 || first >= lo + nb) return false;
+  if (first + row > lo) return true;
+  if (pitch <= 0) return false;
+  const uintptr_t k = (lo - first - row) / (uintptr_t)pitch + 1;  // the first row that ends behind lo
+  return k < (uintptr_t)rows && first + k * (uintptr_t)pitch < lo + nb;
+}
+
 // Four channels a lane where more than half of a wavefront's lanes find work, one otherwise: training
 // pass of 60000 rows, 16-bit, 64 channels 62 us with one and 75 with four, 128 channels 76 and 79, 160
 // channels 97 and 82, 512 channels 209 and 139.  An output over an input allows four only where no
@@ -1100,6 +1110,11 @@ extern "C" int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int lo
       return;
     }
     if (!gate || !x || !out || (!state && num_slots > 0)) return;
+    const size_t state_bytes = (size_t)num_slots * (size_t)channels * 4;
+    auto meets_state = [&](const void* p, int64_t stride, int elem) {
+      return rows_meet(p, batch, stride * elem, (size_t)channels * (size_t)elem, state, state_bytes);
+    };
+    if (meets_state(gate, gate_row_stride, (int)sizeof(TG)) || meets_state(x, x_row_stride, (int)sizeof(TX)) || meets_state(out, out_row_stride, (int)sizeof(TX))) return;
     const int64_t vectors = ceil_div(channels, (int64_t)4), few = ceil_div(vectors, (int64_t)kStepBlock);
     const int64_t wide = ceil_div(vectors, (int64_t)kStepBlock * kStepWide);
     const bool many = batch * wide >= 2 * (int64_t)device_cu_count();

@@ -687,6 +687,13 @@ extern "C" int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const 
   const int64_t entries = (int64_t)c.num_sequences * c.max_pages;
   if (*temp_bytes < bytes || !live_out || !cache_usable(c) || (c.num_pages > 0 && !refs_out) || (entries > 0 && !tables_out))
     return hipErrorInvalidValue;
+  // the outputs may be the cache's own arrays, and meet nothing else
+  const size_t table_bytes = (size_t)entries * 4, ref_bytes = (size_t)c.num_pages * 4, length_bytes = (size_t)c.num_sequences * 4;
+  if ((tables_out != c.tables && ranges_overlap(tables_out, table_bytes, c.tables, table_bytes)) || ranges_overlap(tables_out, table_bytes, c.refs, ref_bytes) ||
+      (refs_out != c.refs && ranges_overlap(refs_out, ref_bytes, c.refs, ref_bytes)) || ranges_overlap(refs_out, ref_bytes, c.tables, table_bytes) ||
+      ranges_overlap(tables_out, table_bytes, refs_out, ref_bytes) || ranges_overlap(tables_out, table_bytes, c.lengths, length_bytes) ||
+      ranges_overlap(refs_out, ref_bytes, c.lengths, length_bytes))
+    return hipErrorInvalidValue;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (c.num_pages == 0) {  // nothing to move; tables name nothing
     hipError_t e = zero_async(live_out, 4, s);

@@ -62,15 +62,15 @@ class Outliving:
         self.tensor, self.device = tensor, device
         self._streams, self._captured = [stream(device)], False
 
-    def used(self):
-        """Before or after a call on the current stream of the device, which is the current one."""
-        if self.device.type != "cuda":
+    def used(self, s):
+        """By a call on stream `s`, the current one of the device, which is the current one."""
+        if self.device.type != "cuda" or s == 0 == self._streams[0]:  # its own; the default stream captures nothing
             return
         if capturing():
             if not self._captured:
                 self._captured = True
                 _CAPTURED.append(self.tensor)
-        elif (s := stream(self.device)) not in self._streams:
+        elif s not in self._streams:
             self.tensor.record_stream(torch.cuda.current_stream(self.device))
             self._streams.append(s)
 

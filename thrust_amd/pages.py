@@ -11,11 +11,6 @@ import torch
 from . import capi, device as dev
 
 
-def _overlap(a, b):
-    """Whether two contiguous tensors of 32 bits share memory."""
-    return a.numel() and b.numel() and a.data_ptr() < b.data_ptr() + 4 * b.numel() and b.data_ptr() < a.data_ptr() + 4 * a.numel()
-
-
 class PageCache:
     """`pools`: the arrays that are paged together (a layer's keys, its values, its recurrent states ...),
     each [pages, ...], contiguous, of any type, with the same number of pages and of bytes a page.  A page
@@ -51,14 +46,15 @@ class PageCache:
         self._tables = self._array(tables, (max_sequences, max_pages), -1, "tables")
         self._lengths = self._array(lengths, (max_sequences,), 0, "lengths")
         self._refs = self._array(refs, (pages,), 0, "refs")
+        self._home = dev.stream(device)
         self._pointers = dev.Outliving(torch.tensor([p.data_ptr() for p in pools], dtype=torch.int64).to(device), device)
         self._args = capi.PageCacheArgs(pools=self._pointers.tensor.data_ptr(), page_bytes=total // max(pages, 1), num_pools=len(pools), num_pages=pages,
                                         page_size=page_size, num_sequences=max_sequences, max_pages=max_pages,
                                         tables=self.tables.data_ptr(), lengths=self.lengths.data_ptr(), refs=self.refs.data_ptr())
         self._ref = ctypes.byref(self._args)
         self._sizes = {}
-        self._own = [self.tables, self.lengths, self.refs]
-        self._all = self._own + pools
+        self._own = (self._tables, self._lengths, self._refs)
+        self._all = (*self._own, *pools)
 
     def _array(self, given, shape, value, what):
         if given is None:
@@ -75,17 +71,18 @@ class PageCache:
                 raise ValueError("requests must be int32 vectors of one length, contiguous")
         return ids[0].shape[0]
 
-    def _temp(self, entry, key, *args):
+    def _temp(self, stream, entry, key, *args):
         """Temporary storage for a call that copies pages: its size asked for once, allocated each time (a graph keeps its own)."""
-        self._pointers.used()
-        nbytes = self._sizes.get(key)
-        if nbytes is None:
+        if stream or self._home:  # on the default stream the allocator's own order does
+            self._pointers.used(stream)
+        size = self._sizes.get(key)
+        if size is None:
             nbytes = ctypes.c_size_t(0)
             capi.check(entry(None, ctypes.byref(nbytes), self._ref, *args, None), key[0] + "(size)")
             if len(self._sizes) > 256:
                 self._sizes.clear()
-            self._sizes[key] = nbytes
-        return dev.empty(self.refs, (nbytes.value,), torch.uint8), ctypes.byref(nbytes)
+            size = self._sizes[key] = (nbytes.value,), ctypes.byref(nbytes)
+        return dev.empty(self._refs, size[0], torch.uint8), size[1]
 
     def resize(self, sequences, lengths):
         """sequences[i] gets the length lengths[i] (int32 tensors).  Pages given up are there for the
@@ -94,11 +91,13 @@ class PageCache:
         before, a length out of range, not enough free pages), which changes nothing of the sequence."""
         n = self._requests(sequences, lengths)
         L = capi.lib()
-        done = dev.empty(self.refs, (n,), torch.bool)
+        done = dev.empty(self._refs, (n,), torch.bool)
         with dev.current(self.device):
-            temp, nbytes = self._temp(L.thrust_cdna4_pages_resize, ("pages_resize", n), None, None, n, None)
-            capi.check(L.thrust_cdna4_pages_resize(temp.data_ptr(), nbytes, self._ref, sequences.data_ptr(), lengths.data_ptr(), n,
-                                                   done.data_ptr(), dev.stream(self.device)), "pages_resize")
+            stream = dev.stream(self.device)
+            temp, nbytes = self._temp(stream, L.thrust_cdna4_pages_resize, ("pages_resize", n), None, None, n, None)
+            rc = L.thrust_cdna4_pages_resize(temp.data_ptr(), nbytes, self._ref, sequences.data_ptr(), lengths.data_ptr(), n, done.data_ptr(), stream)
+        if rc:
+            capi.check(rc, "pages_resize")
         dev.wrote(self._all)
         return done
 
@@ -116,11 +115,14 @@ class PageCache:
         that is not empty, a parent or named before, not enough free pages)."""
         n = self._requests(parents, children)
         L = capi.lib()
-        done = dev.empty(self.refs, (n,), torch.bool)
+        done = dev.empty(self._refs, (n,), torch.bool)
         with dev.current(self.device):
-            temp, nbytes = self._temp(L.thrust_cdna4_pages_fork, ("pages_fork", n), None, None, n, 0, None)
-            capi.check(L.thrust_cdna4_pages_fork(temp.data_ptr(), nbytes, self._ref, parents.data_ptr(), children.data_ptr(), n, bool(share),
-                                                 done.data_ptr(), dev.stream(self.device)), "pages_fork")
+            stream = dev.stream(self.device)
+            temp, nbytes = self._temp(stream, L.thrust_cdna4_pages_fork, ("pages_fork", n), None, None, n, 0, None)
+            rc = L.thrust_cdna4_pages_fork(temp.data_ptr(), nbytes, self._ref, parents.data_ptr(), children.data_ptr(), n, bool(share),
+                                           done.data_ptr(), stream)
+        if rc:
+            capi.check(rc, "pages_fork")
         dev.wrote(self._all)
         return done
 
@@ -132,17 +134,17 @@ class PageCache:
             raise ValueError("tables and refs go together")
         if dev.need_device(tables, refs) not in (None, self.device):
             raise ValueError("tensors on another device than the cache")
-        tables = self.tables if tables is None else self._array(tables, self.tables.shape, None, "tables")
-        refs = self.refs if refs is None else self._array(refs, self.refs.shape, None, "refs")
-        for new, own in ((tables, self.tables), (refs, self.refs)):
-            for t in self._own:
-                if not (t is own and new.data_ptr() == own.data_ptr()) and _overlap(new, t):
-                    raise ValueError("the outputs share memory with the cache's arrays, and are not the same")
+        tables = self._tables if tables is None else self._array(tables, self._tables.shape, None, "tables")
+        refs = self._refs if refs is None else self._array(refs, self._refs.shape, None, "refs")
         L = capi.lib()
-        live = dev.empty(self.refs, (1,), torch.int32)
+        live = dev.empty(self._refs, (1,), torch.int32)
         with dev.current(self.device):
-            temp, nbytes = self._temp(L.thrust_cdna4_pages_compact, ("pages_compact",), None, None, None)
-            capi.check(L.thrust_cdna4_pages_compact(temp.data_ptr(), nbytes, self._ref, tables.data_ptr(), refs.data_ptr(), live.data_ptr(),
-                                                    dev.stream(self.device)), "pages_compact")
-        dev.wrote([tables, refs, *self.pools])
+            stream = dev.stream(self.device)
+            temp, nbytes = self._temp(stream, L.thrust_cdna4_pages_compact, ("pages_compact",), None, None, None)
+            rc = L.thrust_cdna4_pages_compact(temp.data_ptr(), nbytes, self._ref, tables.data_ptr(), refs.data_ptr(), live.data_ptr(), stream)
+        if rc:
+            if rc == 1 and tables is not self._tables:  # hipErrorInvalidValue: what else is refused has been checked
+                raise ValueError("the outputs share memory with each other or the cache's arrays, and are not the same")
+            capi.check(rc, "pages_compact")
+        dev.wrote((tables, refs, *self.pools))
         return live

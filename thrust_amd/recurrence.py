@@ -158,7 +158,7 @@ def linear_scan(gate, x, init=None, offsets=None, log_gate=False, out=None, retu
     args = capi.LinearScanArgs(*fields, *gate_args, *x_args, *out_args, dev.pointer(offsets), dev.pointer(init), final.data_ptr(), dev.pointer(states))
     _run(capi.lib().thrust_cdna4_linear_scan, args, shape[-2], device, x, "linear_scan")
     if given is not None:
-        dev.wrote([given])
+        dev.wrote((given,))
     return (out, final, states) if return_states else (out, final)
 
 
@@ -208,22 +208,18 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
             raise ValueError("more rows than slots")
     elif slots.dtype != torch.int32 or slots.shape != shape[:1] or not slots.is_contiguous():
         raise ValueError("slots must be int32 [batch], contiguous")
-    written = [state]
+    written = (state,)
     if out is None:
         out, out_stride = dev.empty_like(x), channels
     else:
-        written.append(out)
+        written = (state, out)
         if out.dtype != x.dtype:
             raise ValueError("out must have the type of x")
         _distinct(out, "out")
         out_stride = _rows(out, shape, "out")[1]
         _apart(out, (state, slots), (gate, x))
-    gate_stride, x_stride, gate_at, x_at, state_at = _rows(gate, shape, "gate")[1], _rows(x, shape, "x")[1], gate.data_ptr(), x.data_ptr(), state.data_ptr()
-    behind = state_at + num_slots * channels * 4
-    if (gate_at < behind and state_at < gate_at + (batch * gate_stride + channels) * 4) or (x_at < behind and state_at < x_at + (batch * x_stride + channels) * 4):
-        _apart(state, (gate, x))  # asked again, exactly
-    args = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate_at, gate_stride, x_at, x_stride,
-            out.data_ptr(), out_stride, state_at, num_slots, dev.pointer(slots), batch, channels, dev.stream(device))
+    args = (_DT[gate.dtype], _DT[x.dtype], bool(log_gate), gate.data_ptr(), _rows(gate, shape, "gate")[1], x.data_ptr(), _rows(x, shape, "x")[1],
+            out.data_ptr(), out_stride, state.data_ptr(), num_slots, dev.pointer(slots), batch, channels, dev.stream(device))
     entry = capi.lib().thrust_cdna4_linear_scan_step
     if dev.is_current(device):
         rc = entry(*args)
@@ -231,6 +227,7 @@ def linear_scan_step(gate, x, state, slots=None, log_gate=False, out=None):
         with torch.cuda.device(device):
             rc = entry(*args)
     if rc:
+        _apart(state, (gate, x))  # which the call refuses
         capi.check(rc, "linear_scan_step")
     dev.wrote(written)
     return out
