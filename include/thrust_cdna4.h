@@ -261,7 +261,8 @@ int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes, const thru
  * s = slots[i] (NULL: s = i), state[s] = a[i] * state[s] + x[i] and out[i] = state[s].  `state` is F32
  * [num_slots][channels], contiguous, updated in place; `slots` a DEVICE array.  A row whose slot is
  * negative or not below num_slots is padding: its out is zero and no state changes.  Rows of one slot
- * are successive tokens of one sequence and taken in their order.  Needs no temporary storage.  The
+ * are successive tokens of one sequence and taken in their order, for which all slots are compared: time
+ * grows with the square of the batch from some ten thousand rows on (65536 x 1024: 1.0 ms, 0.17 without slots).  Needs no temporary storage.  The
  * arrays must not overlap, except that out may be x or gate itself; a state that meets gate, x or out is refused.
  */
 int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, const void* gate, int64_t gate_row_stride,
@@ -285,7 +286,8 @@ int thrust_cdna4_linear_scan_step(int gate_dtype, int x_dtype, int log_gate, con
  * has done[i] = 0, and so has one with an id out of range or a sequence that an earlier request of the call
  * names already.  What a refused request wanted stays out of reach for the rest of the call: one that
  * needs pages is refused when the pages wanted by it and by all requests before it (refused ones among
- * them) are more than there were free.  Entries of a table that name no page are passed over.
+ * them) are more than there were free.  Requests are compared with one another, so a call's time grows with
+ * the square of their number (1500: 24 us, 65536: 0.4 ms; at most 2^23).  Entries of a table that name no page are passed over.
  */
 typedef struct thrust_cdna4_page_cache {
   const uint64_t* pools;

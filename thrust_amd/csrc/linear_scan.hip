@@ -9,11 +9,11 @@
 //   c <- a_t g_t,
 // starting from the gradient of the final state and ending in the gradient of the initial one.
 //
-// What bounds it: memory.  Each kernel reads and writes every array once, 6 to 14 bytes a value (a large
-// copy reaches 4.75 TB/s on MI355X).  Measured: 131072 rows of 2048 channels, all 16-bit, 307 us, 5.3 TB/s;
-// 8 x 4096 x 2560 with 32-bit logarithms as gates 153 us, 4.4 TB/s, and its gradient 235 us, 5.0 TB/s.  A
-// short call is bound by the trips to memory one behind the other: 8192 rows of 4096 channels 54 us,
-// 3.7 TB/s.
+// What bounds it: memory.  Each kernel reads and writes every array once, 6 to 20 bytes a value (a large
+// copy reaches 6.0 TB/s on MI355X).  Measured: 131072 rows of 2048 channels, all 16-bit, 320 us, 5.0 TB/s;
+// 8 x 4096 x 2560 with 32-bit logarithms as gates 159 us, 4.2 TB/s, and its gradient 249 us, 4.7 TB/s.  A
+// short call is bound by the trips to memory one behind the other: 8192 rows of 4096 channels 56 us,
+// 3.6 TB/s.
 //
 // Split.  A workgroup of 8 wavefronts takes a tile of 8 S rows by 64 VEC channels; wavefront w holds S
 // consecutive rows of it in registers, a lane holds VEC neighbouring channels of each.  One pass over
@@ -25,11 +25,11 @@
 // so results do not vary from run to run.
 //
 // The tile.  S is 16 rows for 16-bit arrays and 8 otherwise: 64 registers of a lane, which leaves two
-// workgroups to a compute unit (128 registers at most).  Half the rows in twice the workgroups took 450 us
-// instead of 408 for the long sequence, twice as many channels in half the rows 816: every halving of
-// the rows doubles the tiles that wait for one another.  80 registers, for three workgroups, spill and
-// took 491.  A first look-back that met in LDS, group maps behind tile maps, took 459 where the present
-// one took 412.
+// workgroups to a compute unit (128 registers at most).  Half the rows in twice the workgroups take 415 us
+// instead of 336 for the long sequence (uniform gates): every halving of the rows doubles the tiles that
+// wait for one another.  Measured in an earlier build, whose first passes took exp of every 16-bit gate and
+// which took 408 us for the same rows: twice as many channels in half the rows 816; 80 registers, for three
+// workgroups, spill: 491; a look-back that met in LDS, group maps behind tile maps: 459.
 //
 // Descriptors.  A map is one 64-bit word (A's bits << 32 | H's bits), stored inverted in a single
 // relaxed agent-scope atomic; NaNs are stored as the canonical one, so no map is the word 0, which
@@ -766,10 +766,12 @@ __global__ __launch_bounds__(kLinBlock) __attribute__((amdgpu_waves_per_eu(4))) 
 // ---------------------------------------------------------------------------------------
 // One token for each of a batch: state[slot] = a state[slot] + x, out = state.  Rows of one slot are
 // taken in their order: the first of them does all, the others leave.  What bounds it is memory: 2048
-// rows of 8192 16-bit channels take 47 us, 5.0 TB/s.  To know whether a row is the first of its slot a
+// rows of 8192 16-bit channels take 46 us, 5.1 TB/s.  To know whether a row is the first of its slot a
 // workgroup reads all slots, 16 bytes a thread; with one wavefront reading 4 bytes a lane, and four
 // times as many workgroups, the same batch took 89 us.  So a thread takes UNITS = 4 vectors where that
-// leaves two workgroups to a compute unit, and one in a small batch (8 x 1024: 3.5 us on the device).
+// leaves two workgroups to a compute unit, and one in a small batch (8 x 1024: 3.7 us on the device).  The
+// slots read grow with the square of the batch: 16384 rows of 1024 channels take 115 us, 53 without slots;
+// 65536 rows 1027 and 174.
 // ---------------------------------------------------------------------------------------
 constexpr int kStepBlock = 256;
 constexpr int kStepWide = 4;  // vectors a thread takes in a large batch
@@ -949,10 +951,15 @@ inline bool rows_meet(const void* a, int64_t rows, int64_t pitch, size_t row, co
   return k < (uintptr_t)rows && first + k * (uintptr_t)pitch < lo + nb;
 }
 
-// Four channels a lane where more than half of a wavefront's lanes find work, one otherwise: training
-// pass of 60000 rows, 16-bit, 64 channels 62 us with one and 75 with four, 128 channels 76 and 79, 160
-// channels 97 and 82, 512 channels 209 and 139.  An output over an input allows four only where no
-// vector reaches over a workgroup's channels: the neighbour may have replaced what it repeats.
+// Four channels a lane where more than half of a wavefront's lanes find work, one otherwise.  Training pass
+// of 60000 rows, us with one channel a lane and with four (two in the gradient of 32-bit arrays):
+//   channels            64         128        160        192        256        512
+//   16-bit            71,  87    86,  91   112,  93   111,  94   134,  99   232, 151
+//   f32 gates, bf16   85,  98    94, 103   121, 106   122, 109   145, 120   263, 185
+//   32-bit            92,  92    92, 102   111, 125   118, 129   151, 141   262, 239
+// An output over an input allows four only where no vector reaches over a workgroup's channels: the
+// neighbour may have replaced what it repeats.  32768 x 2047 in place takes 161 us so, into a new array 122;
+// in 32 bits 245 and 185.
 inline bool lin_narrow(int64_t channels, bool in_place) { return channels <= 128 || (in_place && channels % 4 != 0); }
 
 }  // namespace tcd
@@ -1036,7 +1043,9 @@ extern "C" int thrust_cdna4_linear_scan_backward(void* temp, size_t* temp_bytes,
     using TG = decltype(tg);
     using TX = decltype(tx);
     LinPlan l;
-    constexpr int kWide = sizeof(TX) == 4 ? 2 : 4;  // the payload of a lane: three arrays of 8 rows
+    // the payload of a lane, three arrays of 8 rows: 8 x 4096 x 2560 in 32 bits, both ways, 533 us with two
+    // channels, 548 with one, 607 with four, which spill
+    constexpr int kWide = sizeof(TX) == 4 ? 2 : 4;
     if (!lin_plan(a->batch, a->rows, a->channels, kLinChunk, lin_narrow(a->channels, false) ? 1 : kWide, l)) return;
     if (temp == nullptr) {
       *temp_bytes = l.bytes;

@@ -7,11 +7,12 @@
 // Nothing depends on the order in which workgroups run.
 //
 // What bounds it: with data to move, memory, each byte read and written once (500 forks of 48 pools,
-// 786 MB: 155 us of copying, 5.1 TB/s, and 14 us of the launches before it; 16 KiB a workgroup at a time,
+// 786 MB: 153 us of copying, 5.1 TB/s, and 14 us of the launches before it; 16 KiB a workgroup at a time,
 // four 16-byte loads of a thread in flight).  Without, the launches: 1500 sequences freed and replaced on
-// 2^20 pages 28.6 us in five, of which listing 4 MB of counts is 6; a cache of up to 8192 pages with up to
-// 64 requests is planned by one workgroup in one launch (9 sequences replaced on 300 pages: 24 us in five
-// launches, 16 in three).
+// 2^20 pages 27.4 us in five, of which listing 4 MB of counts is 6; a cache of up to 8192 pages with up to
+// 64 requests is planned by one workgroup in one launch (9 sequences replaced on 300 pages: three launches
+// instead of five, 16 us instead of 24 when that was done).  Every request is compared with all before it:
+// 16384 take 66 us, 65536 387.
 #include "lm_types.h"
 
 namespace tcd {
