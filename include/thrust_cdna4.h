@@ -206,8 +206,9 @@ int thrust_cdna4_histogram_even(void* temp, size_t* temp_bytes, int sample_dtype
  *
  * Infinities and NaNs stay in their channel and sequence.  Products of factors have an exponent of their
  * own: a state that is a normal number from row to row comes out as one, also where the product of the
- * gates between leaves 32 bits; a state that leaves them on the way is 0 or infinite from there on.  What up
- * to 1024 rows make of a state of zero is summed apart: where these terms alone overflow and only the
+ * gates between leaves 32 bits.  A state that leaves them on the way is 0 or infinite there; whether rows
+ * behind it go on from that or from the product that brings it back depends on where tiles begin.  What up to
+ * 1024 rows make of a state of zero is summed apart: where these terms alone overflow and only the
  * state that enters would cancel them, the result is infinite or NaN.  Results are the same from run to run: what is combined with what
  * depends on the sizes alone.  Temporary storage as for thrust_cdna4_scan; up to
  * THRUST_CDNA4_LINEAR_SCAN_CHUNK rows need none, and then only a non-null address and a size of 256.

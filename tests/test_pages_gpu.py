@@ -612,3 +612,14 @@ def test_a_graph_outlives_the_cache_that_it_was_captured_with():
         assert get(done).tolist() == [True] == ref.fork([0], [1], False)
         assert get(own[0]).tolist() == ref.tables and get(own[1]).tolist() == ref.lengths and get(own[2]).tolist() == ref.refs
         assert all(torch.equal(get(p), q) for p, q in zip(own[3], ref.pools))
+
+
+def test_compact_into_an_empty_view_of_something_else():
+    """A table without entries meets nothing, wherever it points."""
+    counts = ints([0, 2, 0, 1, 0])
+    pool = put(torch.arange(10.0).view(5, 2))
+    cache = thrust_amd.PageCache([pool], 4, 3, 0, refs=counts)
+    new = ints([7] * 5)
+    assert get(cache.compact(tables=counts[2:2].view(3, 0), refs=new)).tolist() == [2]
+    assert get(new).tolist() == [1, 2, 0, 0, 0] and get(counts).tolist() == [0, 2, 0, 1, 0]
+    assert get(pool)[:2].tolist() == [[6.0, 7.0], [2.0, 3.0]]

@@ -690,10 +690,11 @@ extern "C" int thrust_cdna4_pages_compact(void* temp, size_t* temp_bytes, const 
     return hipErrorInvalidValue;
   // the outputs may be the cache's own arrays, and meet nothing else
   const size_t table_bytes = (size_t)entries * 4, ref_bytes = (size_t)c.num_pages * 4, length_bytes = (size_t)c.num_sequences * 4;
-  if ((tables_out != c.tables && ranges_overlap(tables_out, table_bytes, c.tables, table_bytes)) || ranges_overlap(tables_out, table_bytes, c.refs, ref_bytes) ||
-      (refs_out != c.refs && ranges_overlap(refs_out, ref_bytes, c.refs, ref_bytes)) || ranges_overlap(refs_out, ref_bytes, c.tables, table_bytes) ||
-      ranges_overlap(tables_out, table_bytes, refs_out, ref_bytes) || ranges_overlap(tables_out, table_bytes, c.lengths, length_bytes) ||
-      ranges_overlap(refs_out, ref_bytes, c.lengths, length_bytes))
+  auto meet = [](const void* a, size_t na, const void* b, size_t nb) { return na && nb && ranges_overlap(a, na, b, nb); };
+  if ((tables_out != c.tables && meet(tables_out, table_bytes, c.tables, table_bytes)) || meet(tables_out, table_bytes, c.refs, ref_bytes) ||
+      (refs_out != c.refs && meet(refs_out, ref_bytes, c.refs, ref_bytes)) || meet(refs_out, ref_bytes, c.tables, table_bytes) ||
+      meet(tables_out, table_bytes, refs_out, ref_bytes) || meet(tables_out, table_bytes, c.lengths, length_bytes) ||
+      meet(refs_out, ref_bytes, c.lengths, length_bytes))
     return hipErrorInvalidValue;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (c.num_pages == 0) {  // nothing to move; tables name nothing
