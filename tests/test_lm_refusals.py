@@ -373,3 +373,11 @@ def test_compact_refuses_outputs_that_meet_the_caches_arrays(any_device, monkeyp
     for tables, refs in ((rows[1:], Z(3).int()), (Z(4, 2).int(), counts[2:5]), (Z(4, 2).int(), rows.flatten()[:3])):
         with pytest.raises(ValueError, match="share memory"):
             cache.compact(tables=tables, refs=refs)
+
+
+def test_addresses_are_compared_on_the_host():
+    """Whatever torch's default device is."""
+    from thrust_amd import recurrence
+    b = torch.zeros(9, 12)
+    with torch.device("meta"):
+        assert recurrence._meet(b[1:7, :4], b[0:6, :4]) and not recurrence._meet(b[1:7, :4], b.as_strided((3, 2, 4), (24, 12, 1), 4))

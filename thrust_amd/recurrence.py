@@ -47,10 +47,10 @@ def _span(t):
 
 def _rows_at(t):
     """The addresses at which the rows of t begin, ascending, and the bytes of one."""
-    at = torch.tensor([t.data_ptr()])
+    at = torch.tensor([t.data_ptr()], device="cpu")
     for n, s in zip(t.shape[:-1], t.stride()[:-1]):
         if n > 1 and s > 0:
-            at = (at[:, None] + torch.arange(n) * (s * t.element_size())).flatten()
+            at = (at[:, None] + torch.arange(n, device="cpu") * (s * t.element_size())).flatten()
     return at.sort().values, t.shape[-1] * t.element_size()
 
 
